@@ -114,6 +114,14 @@ _SIGNATURES = {
         "li_sample_call": [P, c_char_p, P, P, P, I, I, P, L],
         "li_sample_prepare": [P, I, P, I, P, P, P, P],
     },
+    "logprobs": {
+        "li_token_logprobs": [P, L, P, I, I, I, P, P, P, P, P],
+    },
+    "evict": {
+        "li_attention_mass": [P, I, P, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P],
+        "li_evict_select": [P, P, I, P, P, I, I, I, P, I, I, I, I, I],
+        "li_cache_compact": [P, P, I, P, I, P, I, I, I, I, I, I],
+    },
 }
 _fn_cache = {}
 
@@ -1927,6 +1935,140 @@ def sample_prepare(rows: torch.Tensor, table: torch.Tensor, temperature: torch.T
     if n:
         _run("sampling", "li_sample_prepare", rows.data_ptr(), n, table.data_ptr(), table.shape[0],
              temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), uniform.data_ptr())
+
+
+# ------------------------------------------------------------------ log probabilities of given tokens
+LOGPROBS_MAX_TOP = 32                  # alternatives a row
+LOGPROBS_MAX_VOCAB = 1 << 20
+
+
+def _one_device(what: str, *ts) -> None:
+    """The kernels run on the current device and stream: tensors of another one are refused."""
+    here = _get_device() if _get_device is not None else torch.cuda.current_device()
+    _chk(all(t is None or t.device.index == here for t in ts), f"{what}: all tensors have to be on the current device, cuda:{here}")
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, entropy: torch.Tensor,
+                   top_ids: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None) -> None:
+    """For every row x of `logits` [n, V] (float32; rows may be further apart than V): logprobs[i] = x[ids[i]] - log(sum(exp(x))), the entropy of
+    the row's distribution in nats, and, with `top_ids` (int32) and `top_logprobs` (float32) [n, k], k up to LOGPROBS_MAX_TOP, its k likeliest
+    tokens in falling order, the lower id first on ties.  Logits of -inf have no probability: log probability -inf, no share of the entropy.  An id
+    outside the row gives NaN.  A row whose largest logit is not finite, or that holds a NaN, gives NaN throughout; its top ids are ordered with
+    NaN as -inf."""
+    _gpu(logits, ids, logprobs, entropy, top_ids, top_logprobs)
+    _one_device("token_logprobs", logits, ids, logprobs, entropy, top_ids, top_logprobs)
+    _chk(_rows_ok(logits) and logits.dtype is torch.float32, "token_logprobs: logits must be float32 rows [n, V]")
+    n, v = logits.shape
+    _chk(ids.dtype is torch.int32 and ids.shape == (n,) and ids.is_contiguous(), "token_logprobs: ids must be int32 [n]")
+    for t in (logprobs, entropy):
+        _chk(t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous(), "token_logprobs: logprobs and entropy must be float32 [n]")
+    _chk((top_ids is None) == (top_logprobs is None), "token_logprobs: top_ids and top_logprobs go together")
+    top = 0
+    if top_ids is not None:
+        _chk(top_ids.dim() == 2 and top_ids.shape[0] == n and top_ids.dtype is torch.int32 and top_ids.is_contiguous() and top_logprobs.shape == top_ids.shape
+             and top_logprobs.dtype is torch.float32 and top_logprobs.is_contiguous(), "token_logprobs: top_ids int32 and top_logprobs float32 [n, k]")
+        top = top_ids.shape[1]
+        _chk(top <= min(LOGPROBS_MAX_TOP, v), f"token_logprobs: {top} alternatives of {v} tokens (at most {LOGPROBS_MAX_TOP})")
+    _chk(0 < v <= LOGPROBS_MAX_VOCAB, f"token_logprobs: rows of {v} logits (1 to {LOGPROBS_MAX_VOCAB})")
+    if n:
+        work = _scratch.floats(_logprobs_work_floats(n, v), logits.device)
+        _run("logprobs", "li_token_logprobs", logits.data_ptr(), logits.stride(0), ids.data_ptr(), n, v, top, logprobs.data_ptr(), entropy.data_ptr(),
+             top_ids.data_ptr() if top else 0, top_logprobs.data_ptr() if top else 0, work.data_ptr())
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_work_floats(n: int, v: int) -> int:
+    return int(_lib_fn("logprobs", "li_token_logprobs_work_floats", [c_int, c_int], c_long)(n, v))
+
+
+# ------------------------------------------------------------------ a cache of bounded length
+def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta, nh: int, nkv: int, dh: int, page_size: int, scale: float,
+                   fresh: bool = True, ws=None) -> None:
+    """The attention weight that every cached key draws of the batch's queries is added up beside the keys: mass[t, g] += the sum, over the queries
+    that see key t and the heads of kv head g, of softmax(scale q . k)[t].  Queries are heads 0..nh-1 of qkv's rows; `meta` is the batch as
+    `paged_attention` takes it (a query sees the keys up to its own place); mass [pages, nkv, page_size, 1] float32 lies in the keys' pages.  With
+    `fresh` the sums of the keys that this step wrote begin at zero (whatever the pages held); an entry that reads another's keys adds to all.
+    Sums are float32 in an order that depends on the batch alone.  `ws` lends the buffers."""
+    _gpu(qkv, mass, k, meta.block_table)
+    _one_device("attention_mass", qkv, mass, k, meta.block_table, meta.q_start, meta.q_len, meta.ctx_len)
+    check_attention_sizes(nh, nkv, dh)
+    _check_qkv(qkv, nh, dh)
+    _check_cache(k, k, nkv, dh, page_size, qkv.dtype)
+    _chk(mass.dtype is torch.float32 and mass.shape == (k.shape[0], nkv, page_size, 1) and mass.is_contiguous(),
+         "attention_mass: mass must be float32 [pages, kv_heads, page_size, 1]")
+    t, bt, n = qkv.shape[0], meta.block_table, meta.num_segments
+    _chk(t == meta.num_tokens, "attention_mass: batch metadata is of another batch")
+    _chk(bt.dtype is torch.int32 and bt.shape == (n, meta.max_blocks) and bt.is_contiguous(), "attention_mass: block table")
+    _chk(all(x.dtype is torch.int32 and x.numel() == n and x.is_contiguous() for x in (meta.q_start, meta.q_len, meta.ctx_len)),
+         "attention_mass: q_start, q_len and ctx_len must be int32 [segments]")
+    _chk(meta.max_blocks * page_size >= meta.max_ctx_len, "attention_mass: block table too short")
+    if not t:
+        return
+    # (a recorded step is replayed for longer contexts of the same tables)
+    keys = meta.max_blocks * page_size if meta.padded else meta.max_ctx_len
+    need = int(_lib_fn("evict", "li_attention_mass_work_floats", [c_int, c_int], c_long)(t, nh))
+    work = ws.buffer("evict.mass", (need,), torch.float32) if ws is not None else _scratch.floats(need, qkv.device)
+    _run("evict", "li_attention_mass", qkv.data_ptr(), qkv.stride(0), k.data_ptr(), mass.data_ptr(), _DT[qkv.dtype], bt.data_ptr(), meta.max_blocks,
+         meta.q_start.data_ptr(), meta.q_len.data_ptr(), meta.ctx_len.data_ptr(), n, meta.max_q_len, keys, nh, nkv, dh, page_size, k.shape[0],
+         float(scale), int(bool(fresh)), work.data_ptr())
+
+
+def _check_requests(what: str, block_table, n: int, page_size: int) -> None:
+    _chk(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n and block_table.shape[1] > 0
+         and block_table.is_contiguous(), f"{what}: block_table must be int32 [requests, blocks]")
+    _chk(block_table.shape[1] * page_size < 1 << 31, f"{what}: more than 2^31 places a request")
+
+
+def evict_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, first: int, recent: int, out: torch.Tensor) -> None:
+    """Which places of the cache stay, for every entry, request and kv head: of the lens[i] places of request i, min(keep[i], lens[i]) (and no more
+    than `out` has room for): the last `recent` of them, the first `first` (as far as these are not too many), and of the others those with the
+    largest sums, the lower place first on ties (a sum of NaN after all others).  mass [entries, pages, kv_heads, page_size, 1] float32;
+    block_table int32 [requests, blocks]; lens, keep int32 [requests]; out int32 [entries, requests, kv_heads, K]: the places in rising
+    order, -1 behind the last."""
+    _gpu(mass, block_table, lens, keep, out)
+    _one_device("evict_select", mass, block_table, lens, keep, out)
+    _chk(mass.dim() == 5 and mass.shape[4] == 1 and mass.dtype is torch.float32 and mass.is_contiguous(),
+         "evict_select: mass must be float32 [entries, pages, kv_heads, page_size, 1]")
+    entries, pages, nkv, page_size, _ = mass.shape
+    n = lens.numel()
+    _chk(all(x.dtype is torch.int32 and x.shape == (n,) and x.is_contiguous() for x in (lens, keep)), "evict_select: lens and keep must be int32 [requests]")
+    _check_requests("evict_select", block_table, n, page_size)
+    _chk(first >= 0 and recent >= 0, "evict_select: first and recent must not be negative")
+    _chk(out.dtype is torch.int32 and out.dim() == 4 and out.shape[:3] == (entries, n, nkv) and out.is_contiguous(),
+         "evict_select: out must be int32 [entries, requests, kv_heads, K]")
+    _chk(entries <= 65535 and n <= 65535, "evict_select: at most 65,535 entries and requests")
+    if out.numel():
+        _run("evict", "li_evict_select", mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], lens.data_ptr(), keep.data_ptr(), n,
+             min(int(first), 1 << 30), min(int(recent), 1 << 30), out.data_ptr(), out.shape[3], entries, nkv, page_size, pages)
+
+
+CACHE_COMPACT_MAX_TENSORS = 4
+
+
+def cache_compact(tensors, block_table: torch.Tensor, kept: torch.Tensor) -> None:
+    """The kept places of every entry, request and kv head move to the front: row j of a request's rows becomes what row kept[.., j] was, for
+    all tensors alike; rows behind the last kept one stay as they were.  tensors: up to CACHE_COMPACT_MAX_TENSORS of [entries, pages,
+    kv_heads, page_size, size] with rows of whole 4 bytes; block_table int32 [requests, blocks], no page in two rows; kept int32
+    [entries, requests, kv_heads, K] in rising order, -1 behind the last (as `evict_select` leaves it).  A place beyond the table, or on a page
+    that the table does not have, is not moved."""
+    tensors = list(tensors)
+    _gpu(*tensors, block_table, kept)
+    _one_device("cache_compact", *tensors, block_table, kept)
+    _chk(1 <= len(tensors) <= CACHE_COMPACT_MAX_TENSORS, f"cache_compact: 1 to {CACHE_COMPACT_MAX_TENSORS} tensors")
+    _chk(kept.dim() == 4 and kept.dtype is torch.int32 and kept.is_contiguous(), "cache_compact: kept must be int32 [entries, requests, kv_heads, K]")
+    entries, n, nkv, most = kept.shape
+    _chk(all(t.dim() == 5 and t.is_contiguous() and t.shape[0] == entries and t.shape[2] == nkv and t.shape[1:4] == tensors[0].shape[1:4]
+             and t.shape[4] * t.element_size() % 4 == 0 for t in tensors),
+         "cache_compact: tensors must be contiguous [entries, pages, kv_heads, page_size, size] with rows of whole 4 bytes")
+    pages, _, page_size = tensors[0].shape[1:4]
+    _check_requests("cache_compact", block_table, n, page_size)
+    _chk(entries <= 65535 and n <= 65535, "cache_compact: at most 65,535 entries and requests")
+    if kept.numel() and all(t.numel() for t in tensors):
+        count = len(tensors)
+        at = (c_void_p * count)(*(t.data_ptr() for t in tensors))
+        rows = (c_int * count)(*(t.shape[4] * t.element_size() for t in tensors))
+        _run("evict", "li_cache_compact", ctypes.addressof(at), ctypes.addressof(rows), count, block_table.data_ptr(), block_table.shape[1],
+             kept.data_ptr(), most, n, entries, nkv, page_size, pages)
 
 
 # ------------------------------------------------------------- position vector, logits, pages, map difference
