@@ -2,6 +2,7 @@
 
     python -m litinfer_amd generate --model DIR --prompt-ids 1,2,3 --max_steps 32
     python -m litinfer_amd generate --random config.json --seed 0 --prompt-ids 1,2,3
+    python -m litinfer_amd score --model DIR --prompt-ids 1,2,3 --top 5
     python -m litinfer_amd random   --config config.json --seed 0 --out DIR
     python -m litinfer_amd replay   --model DIR --dtype float32 --out DIR --max-tokens 256 < steps.jsonl
     python -m litinfer_amd bench    [the options of bench.py]
@@ -21,15 +22,16 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import sys
 
 
 def _cmd_generate(a) -> int:
     from .models import load
-    if a.test:
+    if getattr(a, "test", False):
         a.top_p, a.top_k, a.temperature = 1.0, 1, 1.0
     if (a.model is None) == (a.random is None):
-        print("generate: give either --model DIR or --random CONFIG.json", file=sys.stderr)
+        print(f"{a.cmd}: give either --model DIR or --random CONFIG.json", file=sys.stderr)
         return 2
     tmp = None
     if a.random is not None:                      # random weights of that configuration, written to a folder that goes again
@@ -59,14 +61,20 @@ def _generate(a, load) -> int:
         from pathlib import Path
         tok_path = Path(a.model) / "tokenizer.json"
         if not tok_path.exists():
-            print("generate: --prompt needs tokenizer.json in the model folder; "
+            print(f"{a.cmd}: --prompt needs tokenizer.json in the model folder; "
                   "use --prompt-ids instead", file=sys.stderr)
             return 2
         from tokenizers import Tokenizer
         tokenizer = Tokenizer.from_file(str(tok_path))
         ids = tokenizer.encode(a.prompt).ids
     model = load(a.model, device=a.device, dtype=a.dtype, page_size=a.page_size, num_pages=a.num_pages,
-                 max_batch_tokens=a.max_batch_tokens, chunk_size=a.chunk_size, seed=a.seed)
+                 max_batch_tokens=a.max_batch_tokens, chunk_size=a.chunk_size, seed=getattr(a, "seed", 0), cache_budget=a.cache_budget)
+    if a.cmd == "score":
+        rows = model.score(ids, top=a.top)
+        total = sum(r.logprob for r in rows)
+        print(json.dumps({"tokens": len(rows), "logprob": total, "perplexity": math.exp(-total / len(rows)) if rows else None,
+                          "rows": [{"token": r.token, "logprob": r.logprob, "entropy": r.entropy, "top": [list(t) for t in r.top]} for r in rows]}))
+        return 0
     tokens, metrics = model.generate_profile(ids, max_new_tokens=a.max_steps, top_k=a.top_k,
                                              top_p=a.top_p, temperature=a.temperature)
     print(json.dumps({"tokens": tokens, **{k: round(v, 6) if isinstance(v, float) else v
@@ -112,26 +120,31 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m litinfer_amd")
     sub = ap.add_subparsers(dest="cmd", required=True)
     g = sub.add_parser("generate", help="generate tokens from a prompt")
-    g.add_argument("--model", default=None, type=str)
-    g.add_argument("--random", default=None, type=str, metavar="CONFIG.json",
-                   help="instead of --model: random weights for this configuration")
-    g.add_argument("--weights-seed", default=0, type=int, help="seed of the random weights (--random)")
-    g.add_argument("--device", default="cuda:0", type=str)
-    g.add_argument("--prompt", default="Who are you?", type=str)
-    g.add_argument("--prompt-ids", default=None, type=str, help="token ids, comma or space separated")
-    g.add_argument("--prompt-file", default=None, type=str, help="JSON list of token ids")
+    sc = sub.add_parser("score", help="log probabilities of a given text's tokens")
+    for q in (g, sc):
+        q.add_argument("--model", default=None, type=str)
+        q.add_argument("--random", default=None, type=str, metavar="CONFIG.json",
+                       help="instead of --model: random weights for this configuration")
+        q.add_argument("--weights-seed", default=0, type=int, help="seed of the random weights (--random)")
+        q.add_argument("--device", default="cuda:0", type=str)
+        q.add_argument("--prompt", default="Who are you?", type=str)
+        q.add_argument("--prompt-ids", default=None, type=str, help="token ids, comma or space separated")
+        q.add_argument("--prompt-file", default=None, type=str, help="JSON list of token ids")
+        q.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+        q.add_argument("--page-size", default=16, type=int)
+        q.add_argument("--num-pages", default=None, type=int)
+        q.add_argument("--max-batch-tokens", default=2048, type=int)
+        q.add_argument("--chunk-size", default=512, type=int)
+        q.add_argument("--cache-budget", default=None, type=int, metavar="N",
+                       help="cut a request's cache to the N tokens that drew most attention when it has grown beyond")
+        q.set_defaults(fn=_cmd_generate)
+    sc.add_argument("--top", default=0, type=int, help="likeliest tokens to show at every place")
     g.add_argument("--max_steps", "--max-new-tokens", dest="max_steps", default=128, type=int)
     g.add_argument("--top_p", "--top-p", dest="top_p", default=0.8, type=float)
     g.add_argument("--top_k", "--top-k", dest="top_k", default=50, type=int)
     g.add_argument("--temperature", default=1.0, type=float)
     g.add_argument("--test", action="store_true", help="greedy: top_p=1, top_k=1, temperature=1")
     g.add_argument("--seed", "--sample-seed", dest="seed", default=0, type=int, help="seed of the sampler")
-    g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
-    g.add_argument("--page-size", default=16, type=int)
-    g.add_argument("--num-pages", default=None, type=int)
-    g.add_argument("--max-batch-tokens", default=2048, type=int)
-    g.add_argument("--chunk-size", default=512, type=int)
-    g.set_defaults(fn=_cmd_generate)
     r = sub.add_parser("random", help="write a model folder with random weights")
     r.add_argument("--config", required=True)
     r.add_argument("--seed", type=int, default=0)

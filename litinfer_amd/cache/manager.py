@@ -295,6 +295,19 @@ class CacheManager:
         self._lib.li_book_cached_many(self._book, len(handles), handles.ctypes.data, out.ctypes.data)
         return np.maximum(out, 0)
 
+    def positions_many(self, handles) -> "np.ndarray":
+        """The position of each request's next token: its cached tokens and those that were evicted (0 for a handle < 0)."""
+        out = np.zeros(len(handles), dtype=np.int32)
+        self._lib.li_book_positions_many(self._book, len(handles), handles.ctypes.data, out.ctypes.data)
+        return out
+
+    def evict_many(self, handles, keep: int) -> None:
+        """Only `keep` tokens of each request are left, in the first places (their rows have been moved there); pages behind them go
+        back, and the requests' next tokens stand at the positions where they would have stood."""
+        handles = np.ascontiguousarray(handles, dtype=np.int64)
+        if self._lib.li_book_evict_many(self._book, len(handles), handles.ctypes.data, int(keep)) < 0:
+            raise ValueError(self._error())
+
     def max_table_len(self, handles) -> List[int]:
         """The longest block table among the requests, per group."""
         if self._lib.li_book_max_table_len(self._book, len(handles), handles.ctypes.data, self._ints) < 0:
@@ -321,11 +334,18 @@ class CacheManager:
         """Whether any mixer keeps per-request state of fixed size in this cache."""
         return bool(self._entry_state)
 
+    @property
+    def accumulates(self) -> bool:
+        """Whether a step adds to what earlier tokens of a request hold in their pages."""
+        return any(t.accumulates for g in self.groups for t in g.need.tensors)
+
     def rewind(self, rid, n: int) -> None:
         """Forget the last `n` tokens of `rid`: their positions will be computed and written
         again.  The pages stay with the request.  Refused (ValueError) where a windowed group has
         already given back a page that the earlier position still sees, and where any entry keeps
-        state of fixed size: such a state has moved on with the tokens and cannot be taken back."""
+        state of fixed size or adds to what earlier tokens hold: such a state has moved on with the tokens and cannot be taken back."""
+        if n and self.accumulates:
+            raise ValueError("cache: a request's last tokens cannot be forgotten where steps add to what earlier tokens hold")
         if self._entry_state and n:
             raise ValueError("cache: a request's last tokens cannot be forgotten where a mixer keeps state of fixed "
                              "size (the state has moved on with them)")

@@ -78,7 +78,8 @@ struct Pool {
 
 struct Request {
     int slot = 0;
-    int cached = 0;
+    int cached = 0;                            // places of the cache that hold a token
+    int evicted = 0;                           // tokens that were dropped from between the cached ones: the next one stands at cached + evicted
     std::vector<std::vector<int>> tables;      // per group: logical block -> page or -1
     std::vector<int> first_live;               // per group: first block not yet given back
 };
@@ -360,6 +361,41 @@ int li_book_rewind(void* vb, int64_t h, int n) {
     r->cached -= n;
     return 0;
 }
+// Only `keep` of the cached tokens are left, in the first places; pages behind them go back.  Refused where a group gives pages back by
+// position: its window or chunk counts places as positions.
+int li_book_evict_many(void* vb, int n, const int64_t* handles, int keep) {
+    Book* b = (Book*)vb;
+    if (keep <= 0) return b->fail(ERR_ARG, "cache: at least one token of a request stays");
+    for (size_t g = 0; g < b->pools.size(); ++g)
+        if (b->gives_back((int)g)) return b->fail(ERR_ARG, "cache: tokens cannot be dropped from between those of a windowed or chunked group");
+    for (int i = 0; i < n; ++i) {
+        const Request* r = b->find(handles[i]);
+        if (!r) return b->fail(ERR_UNKNOWN, "cache: unknown request");
+        if (keep > r->cached) return b->fail(ERR_ARG, "cache: cannot keep " + std::to_string(keep) + " of " + std::to_string(r->cached) + " cached tokens");
+    }
+    const size_t blocks = (size_t)((keep + b->page_size - 1) / b->page_size);
+    for (int i = 0; i < n; ++i) {
+        Request* r = b->find(handles[i]);
+        for (size_t g = 0; g < b->pools.size(); ++g)
+            while (r->tables[g].size() > blocks) {
+                const int rc = b->pools[g].release(r->tables[g].back());
+                if (rc < 0) return b->fail(rc, b->pools[g].error);
+                r->tables[g].pop_back();
+            }
+        r->evicted += r->cached - keep;
+        r->cached = keep;
+    }
+    return 0;
+}
+// Positions that the batch's requests have passed (cached and evicted tokens), out [n] (0 for a request that is not live).
+int li_book_positions_many(void* vb, int n, const int64_t* handles, int* out) {
+    Book* b = (Book*)vb;
+    for (int i = 0; i < n; ++i) {
+        Request* r = handles[i] >= 0 ? b->find(handles[i]) : nullptr;
+        out[i] = r ? r->cached + r->evicted : 0;
+    }
+    return 0;
+}
 int li_book_release(void* vb, int64_t h) {
     Book* b = (Book*)vb;
     auto it = b->requests.find(h);
@@ -492,7 +528,7 @@ long li_book_build_batch(void* vb, int nseg, const int64_t* handles, const int* 
                 ++nt;
             }
         for (int j = 0; j < q_len[i]; ++j, ++t) {
-            d_pos[t] = r->cached + j;
+            d_pos[t] = r->cached + r->evicted + j;
             d_seg[t] = i;
             if (q_len[i] == 1) { if (token_kinds) d_single[ns] = t; ++ns; }
             else { if (token_kinds) d_multi[nm] = t; ++nm; }

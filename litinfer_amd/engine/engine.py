@@ -59,17 +59,21 @@ class Engine:
                  max_seqs: int = 64, page_order_seed: Optional[int] = None,
                  config: Any = None, use_graphs: bool = True, graph_after: int = 2,
                  keep_stored_precision: bool = False, max_graphs: int = 64, step_tokens: int = 2048,
-                 pad_rows_to: int = 4):
+                 pad_rows_to: int = 4, attention_mass: bool = False):
         """keep_stored_precision: with dtype bfloat16, leave matrices that the checkpoint stores in
         32-bit or half precision in 32-bit (their products then run in the 32-bit kernels) instead of
-        rounding them once to bfloat16 when they are bound."""
+        rounding them once to bfloat16 when they are bound.
+        attention_mass: keep, beside every cached key, the attention weight that it has drawn, so that `evict`
+        can cut a request's cache to the tokens that drew most (models whose every layer attends over all its keys and values)."""
         self.spec = spec
         self.config = config
-        self.rt = Runtime(torch.device(device), parse_dtype(dtype), bool(keep_stored_precision))
+        self.rt = Runtime(torch.device(device), parse_dtype(dtype), bool(keep_stored_precision), attention_mass=bool(attention_mass))
         if self.rt.device.type == "cuda":
             from ..kernels import ops
             ops.require_gpu(self.rt.device)
         self.model = Model(spec, self.rt)
+        if self.rt.attention_mass:
+            self._check_evictable()
         self.page_size = int(page_size)
         self.max_seqs = int(max_seqs)
         self._num_pages = num_pages
@@ -80,6 +84,7 @@ class Engine:
         self.cache: Optional[CacheManager] = None
         self.ws = Workspace(self.rt.device)
         self._uploader = BatchUploader(self.rt.device)
+        self._evict_up = BatchUploader(self.rt.device)
         # ids of tokens chosen on the device (a sampler's output): an entry of the NEXT step may
         # take its token from here (`StepEntry.take`), so the host need not wait for the number
         self.feedback = torch.zeros(FEEDBACK_SLOTS, dtype=torch.int32, device=self.rt.device)
@@ -192,6 +197,16 @@ class Engine:
                                   max_seqs=self.max_seqs, dtype=self.rt.dtype, device=self.rt.device,
                                   page_order_seed=self._page_order_seed)
 
+    def _check_evictable(self) -> None:
+        """Refuses models of which a token cannot be dropped: state of fixed size, compressed caches, windows and chunks."""
+        from ..parts.base import needs_of
+        needs, sources = self.model.cache_needs()
+        for i, (need, src) in enumerate(zip(needs, sources)):
+            paged, states = needs_of(need)
+            if states or (src is None and paged is not None and (paged.reach or all(t.name != "mass" for t in paged.tensors))):
+                raise ValueError(f"engine: attention_mass needs layers that attend over all their keys and values; entry {i} of "
+                                 f"{self.spec.architecture} keeps {need!r}")
+
     @property
     def row_tile(self) -> int:
         """Rows that the model's kernels take at a time, as its parts report it: what a scheduler
@@ -242,7 +257,7 @@ class Engine:
                 if not 0 <= int(w) < n:
                     raise StepError(f"step: request {e.rid!r} wants logits at place {w} of {n} tokens")
         handles = self.cache.handles_of([e.rid for e in entries])
-        reach = self.cache.cached_many(handles) + counts
+        reach = self.cache.positions_many(handles) + counts
         if int(reach.max()) > self.spec.max_positions:
             i = int(np.argmax(reach))
             raise StepError(f"step: request {entries[i].rid!r} would reach {int(reach[i])} positions, the "
@@ -284,9 +299,9 @@ class Engine:
             # is filled up to the next multiple of `pad_rows_to` with copies of its LAST entry: the
             # copies read the same token, position, pages and table row, write the same key and value
             # to the same place, and their logits are dropped.  Not where a mixer keeps state of fixed
-            # size (a copy would step the state a second time).
+            # size (a copy would step the state a second time), nor where a step adds to earlier tokens' rows.
             n = len(entries)
-            fill = -n % self.pad_rows_to if (n > self.pad_rows_to and not self.cache.has_state) else 0
+            fill = -n % self.pad_rows_to if (n > self.pad_rows_to and not (self.cache.has_state or self.cache.accumulates)) else 0
             if fill:
                 rows = sum(len(e.want) for e in entries)
                 last = entries[-1]
@@ -316,6 +331,42 @@ class Engine:
         cache.commit_many(handles, counts)
         self.steps_run += 1
         return logits
+
+    def evict(self, rids: Sequence[Hashable], keep: int, first: int = 4, recent: Optional[int] = None) -> List[int]:
+        """Cuts the cache of every request in `rids` that holds more than `keep` tokens to `keep` of them: its first `first`, its last `recent` (half
+        of `keep` unless given) and, in every layer and kv head by itself, those that have drawn the most attention so far.  Their keys and values
+        move to the front, pages that are left go back at once, and the request's next tokens stand at the positions where they would have stood.
+        Returns how many tokens each request has left.  Needs an engine with `attention_mass`."""
+        if not self.rt.attention_mass:
+            raise ValueError("evict: the engine keeps no attention weights (Engine(..., attention_mass=True))")
+        keep, first, recent = int(keep), int(first), int(keep) // 2 if recent is None else int(recent)
+        if keep < 1 or first < 0 or recent < 0:
+            raise ValueError(f"evict: keep must be positive, first and recent not negative, found {keep}, {first}, {recent}")
+        if len(set(rids)) != len(rids):
+            raise ValueError("evict: a request appears twice")
+        cache = self.cache
+        held = {rid: cache.cached_len(rid) for rid in rids}          # (an unknown request: KeyError)
+        longer = [rid for rid in rids if held[rid] > keep]
+        if longer:
+            from ..kernels import ops
+            n = len(longer)
+            tables = []
+            for g in range(len(cache.groups)):
+                rows = [cache.block_table(rid, g) for rid in longer]
+                table = np.full((n, max(map(len, rows))), -1, dtype=np.int32)
+                for row, ids in zip(table, rows):
+                    row[:len(ids)] = ids
+                tables.append(table)
+            up = self._evict_up.upload([np.array([held[r] for r in longer], dtype=np.int32), np.full(n, keep, dtype=np.int32), *tables])
+            kept = []
+            for group, table in zip(cache.groups, up[2:]):
+                mass = group.data["mass"]
+                kept.append(torch.empty((mass.shape[0], n, mass.shape[2], keep), dtype=torch.int32, device=mass.device))
+                ops.evict_select(mass, table, up[0], up[1], first, recent, kept[-1])
+            for group, table, places in zip(cache.groups, up[2:], kept):
+                ops.cache_compact(list(group.data.values()), table, places)
+            cache.evict_many(cache.handles_of(longer), keep)
+        return [min(held[rid], keep) for rid in rids]
 
     def finish(self, rid: Hashable) -> None:
         """The request is over: what it holds is given back."""

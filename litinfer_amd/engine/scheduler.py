@@ -41,9 +41,10 @@ from dataclasses import dataclass, field
 from typing import Deque, Dict, Hashable, List, Optional, Sequence, Tuple
 
 import numpy as np
+import torch
 
 from ..cache import CacheFull
-from ..sampling import Sampler, SamplingParams
+from ..sampling import Sampler, SamplingParams, TokenLogprob, check_top
 from .batch import StepEntry
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
@@ -69,6 +70,9 @@ class Request:
     # the state slot and the options that the sampler's table on the device holds for this request
     # (None: not written yet, or the request has given its slot back)
     bound: Optional[Tuple[int, SamplingParams]] = None
+    # how many alternatives are wanted beside each generated token's log probability (None: no log probabilities), and what has come
+    top_logprobs: Optional[int] = None
+    logprobs: List[TokenLogprob] = field(default_factory=list)
 
     @property
     def num_generated(self) -> int:
@@ -105,6 +109,18 @@ class _Ready:
         return self._tokens
 
 
+class _WithLogprobs:
+    """A step's tokens and their log probabilities, both on their way."""
+    def __init__(self, tokens, logprobs):
+        self._pending, self._logprobs = tokens, logprobs
+
+    def result(self):
+        return self._pending.result()
+
+    def logprob(self, row: int, top: int) -> TokenLogprob:
+        return self._logprobs.result()[row].cut(top)
+
+
 @dataclass
 class Planned:
     request: Request
@@ -116,8 +132,13 @@ class Planned:
 class Scheduler:
     def __init__(self, engine, *, max_batch_tokens: int = 2048, chunk_size: int = 512,
                  max_running: Optional[int] = None, eos_token_ids: Optional[Sequence[int]] = None,
-                 sampler=None, lookahead: bool = False, row_tile: Optional[int] = None):
-        """row_tile: rows that the kernels of a step take at a time (the products' tiles).  A step
+                 sampler=None, lookahead: bool = False, row_tile: Optional[int] = None, cache_budget: Optional[int] = None,
+                 cache_slack: int = 128, cache_first: int = 4, cache_recent: Optional[int] = None):
+        """cache_budget: a request whose cache has grown more than `cache_slack` tokens beyond so many after a step is cut to that many
+        (`Engine.evict` with the first `cache_first` and the last `cache_recent`, half of them unless given), between the
+        portions of its prompt too.  Its tokens then depend on how its prompt was cut into portions (and a preempted request, which is computed
+        anew, may go on with others).  None: everything is kept.
+        row_tile: rows that the kernels of a step take at a time (the products' tiles).  A step
         whose tokens number a few more than a multiple of it (up to half a tile) pays for a whole
         tile more: then the last portion of a prompt in the plan that is not the prompt's end gives
         those tokens up to the next step.  1: as planned.  None: what the engine's model says
@@ -126,8 +147,13 @@ class Scheduler:
             row_tile = int(getattr(engine, "row_tile", 1) or 1)
         if max_batch_tokens <= 0 or chunk_size <= 0 or row_tile <= 0:
             raise ValueError("scheduler: max_batch_tokens, chunk_size and row_tile must be positive")
+        if cache_budget is not None and (cache_budget <= 0 or cache_slack < 0 or not engine.rt.attention_mass):
+            raise ValueError("scheduler: a cache_budget is positive, its slack not negative, and the engine keeps attention weights "
+                             "(Engine(..., attention_mass=True))")
         self.engine = engine
         self.cache = engine.cache
+        self.cache_budget = None if cache_budget is None else int(cache_budget)
+        self.cache_slack, self.cache_first, self.cache_recent = int(cache_slack), int(cache_first), cache_recent
         self.max_batch_tokens = int(max_batch_tokens)
         self.chunk_size = int(chunk_size)
         self.row_tile = int(row_tile)
@@ -148,7 +174,10 @@ class Scheduler:
     # ---- submitting -----------------------------------------------------
     def add_request(self, prompt: Sequence[int], max_new_tokens: int = 128,
                     params: Optional[SamplingParams] = None, rid: Hashable = None,
-                    first_token_greedy: bool = False) -> Hashable:
+                    first_token_greedy: bool = False, logprobs: Optional[int] = None) -> Hashable:
+        """logprobs: keep every generated token's log probability and that many alternatives (0: none) in `Request.logprobs`: of
+        the model's own distribution, before temperature and cuts."""
+        logprobs = check_top(logprobs, self.engine.spec.vocab_size, "add_request")
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise ValueError("add_request: inputs must not be empty")
@@ -165,6 +194,8 @@ class Scheduler:
         for g, n in zip(self.cache.groups, need):
             if g.need.reach > 0:                      # there a request goes on token by token if it must
                 n = min(n, -(-g.need.reach // self.cache.page_size) + 1 + -(-g.need.keep_first // self.cache.page_size))
+            elif self.cache_budget is not None:
+                n = min(n, -(-(self.cache_budget + self.cache_slack + 1) // self.cache.page_size))
             if n > g.pool.capacity:
                 raise ValueError(f"add_request: the request needs {n} cache pages, the pool has "
                                  f"{g.pool.capacity}: it could never run")
@@ -175,7 +206,7 @@ class Scheduler:
         elif rid in self.requests and self.requests[rid].state != FINISHED:
             raise ValueError(f"add_request: request id {rid!r} is in use")
         req = Request(rid, prompt, int(max_new_tokens), params, first_token_greedy,
-                      arrival=next(self._arrivals))
+                      arrival=next(self._arrivals), top_logprobs=logprobs)
         self.requests[rid] = req
         self.waiting.append(req)
         return rid
@@ -218,11 +249,13 @@ class Scheduler:
         request's further tokens fill.  A windowed group gives pages back as the window passes them:
         there a request holds at most the window's pages and those of the portion that a step brings
         (up to `chunk_size` tokens) at a time, and that is what has to be free for it; a pool smaller
-        than that serves one request at a time, in shorter portions."""
+        than that serves one request at a time, in shorter portions.  With a `cache_budget` the same holds of
+        the budget, its slack and a portion."""
         P = self.cache.page_size
         portion = self.chunk_size if portion is None else portion
         caps = [min(-(-(g.need.reach - 1 + portion) // P) + 1 + -(-g.need.keep_first // P), g.pool.capacity)
-                if g.need.reach > 0 else None
+                if g.need.reach > 0 else
+                min(-(-(self.cache_budget + self.cache_slack + portion) // P), g.pool.capacity) if self.cache_budget is not None else None
                 for g in self.cache.groups]
         if all(c is None for c in caps):
             return need
@@ -352,6 +385,14 @@ class Scheduler:
                 break
         return plan
 
+    def keep_within_budget(self, rids: Sequence[Hashable]) -> None:
+        """Cuts those of the live requests whose cache has outgrown the budget and its slack."""
+        if self.cache_budget is None:
+            return
+        long = [rid for rid in rids if self.cache.cached_len(rid) > self.cache_budget + self.cache_slack]
+        if long:
+            self.engine.evict(long, self.cache_budget, self.cache_first, self.cache_recent)
+
     # ---- one step ------------------------------------------------------------
     def _ends_with_pending(self, r: Request) -> bool:
         """The token that is still on its way is the request's last, whatever it is."""
@@ -385,6 +426,7 @@ class Scheduler:
         self.steps += 1
         for p in plan:
             p.request.computed += p.n
+        self.keep_within_budget([p.request.rid for p in plan])
         sampled = [p.request for p in plan if p.wants_logits]
         params, counters = [], []
         for r in sampled:
@@ -398,8 +440,9 @@ class Scheduler:
         if not self.lookahead:
             produced: List[Tuple[Hashable, int]] = []
             if sampled:
-                for r, tok in zip(sampled, self._sample(logits, sampled, params, counters, None).result()):
-                    if self._append(r, int(tok)):
+                handle = self._sample(logits, sampled, params, counters, None)
+                for i, (r, tok) in enumerate(zip(sampled, handle.result())):
+                    if self._append(r, int(tok), handle, i):
                         produced.append((r.rid, int(tok)))
             return produced
         handle = self._sample(logits, sampled, params, counters, self.engine.feedback) if sampled else None
@@ -415,6 +458,15 @@ class Scheduler:
         """Tokens for the rows of `logits`.  A sampler with a table on the device gets each row's state
         slot and nothing else: a request's options and stream are written there once, when it first
         samples in its slot (and again should its options change)."""
+        tops = [r.top_logprobs for r in sampled if r.top_logprobs is not None]
+        if not tops:
+            return self._choose(logits, sampled, params, counters, out)
+        if out is None:
+            out = torch.empty(len(sampled), dtype=torch.int32, device=logits.device)
+        tokens = self._choose(logits, sampled, params, counters, out)
+        return _WithLogprobs(tokens, self.sampler.logprobs_async(logits, out[:len(sampled)], max(tops)))
+
+    def _choose(self, logits, sampled: List[Request], params, counters, out):
         sampler = self.sampler
         if getattr(sampler, "table", None) is None:
             if hasattr(sampler, "sample_async"):
@@ -441,20 +493,22 @@ class Scheduler:
         handle, sampled = self._inflight
         self._inflight = None
         produced = []
-        for r, tok in zip(sampled, handle.result()):
+        for i, (r, tok) in enumerate(zip(sampled, handle.result())):
             if r.state == FINISHED:                  # ended meanwhile (an end token one step back, an abort)
                 continue
             r.pending_take = None
-            if self._append(r, int(tok)):
+            if self._append(r, int(tok), handle, i):
                 produced.append((r.rid, int(tok)))
         return produced
 
-    def _append(self, r: Request, tok: int) -> bool:
-        """Apply the finishing rules; True if the token was kept."""
+    def _append(self, r: Request, tok: int, handle=None, row: int = 0) -> bool:
+        """Apply the finishing rules; True if the token was kept (its log probability, if wanted, is row `row` of the step's)."""
         if tok in self.eos:
             self._finish(r, "eos")
             return False
         r.generated.append(tok)
+        if r.top_logprobs is not None:
+            r.logprobs.append(handle.logprob(row, r.top_logprobs))
         if len(r.generated) >= r.max_new_tokens:
             self._finish(r, "length")
         elif len(r.prompt) + len(r.generated) >= self.engine.spec.max_positions:

@@ -16,8 +16,10 @@ import time
 from pathlib import Path
 from typing import Iterator, List, Optional, Sequence
 
-from ..engine import Engine, Scheduler
-from ..sampling import SamplingParams
+import torch
+
+from ..engine import Engine, Scheduler, StepEntry
+from ..sampling import SamplingParams, TokenLogprob, check_top
 
 
 def _is_greedy(top_k: int, top_p: float, temperature: float) -> bool:
@@ -39,7 +41,8 @@ class CausalLM:
                  dtype: str = "bfloat16", page_size: int = 16, num_pages: Optional[int] = None,
                  max_tokens: Optional[int] = None, max_seqs: int = 64, max_batch_tokens: int = 2048,
                  chunk_size: int = 512, seed: int = 0, lookahead: bool = True, strict_weights: bool = False,
-                 keep_stored_precision: bool = False):
+                 keep_stored_precision: bool = False, cache_budget: Optional[int] = None):
+        """cache_budget: cached tokens that a request is cut to when it has grown beyond (`Scheduler`); None keeps all."""
         if quantize is not None:
             raise NotImplementedError("quantized weights are not supported")
         self.model_path = Path(model_path)
@@ -47,12 +50,12 @@ class CausalLM:
         self.engine = Engine.from_dir(self.model_path, dtype=dtype, device=device, page_size=page_size,
                                       num_pages=num_pages, max_tokens=max_tokens, max_seqs=max_seqs,
                                       strict_weights=strict_weights, keep_stored_precision=keep_stored_precision,
-                                      step_tokens=max_batch_tokens)
+                                      step_tokens=max_batch_tokens, attention_mass=cache_budget is not None)
         self.meta = self.engine.config
         self.seed = int(seed)
         # lookahead: a step is started before the tokens of the one before have reached the host
         self._sched_args = dict(max_batch_tokens=max_batch_tokens, chunk_size=chunk_size,
-                                lookahead=bool(lookahead))
+                                lookahead=bool(lookahead), cache_budget=cache_budget)
         self._scheduler: Optional[Scheduler] = None
         print(f"[litinfer_amd] ready: {self.engine.spec.architecture}, "
               f"{self.engine.model.weight_bytes() / 2**20:.1f} MiB of weights", flush=True)
@@ -124,6 +127,26 @@ class CausalLM:
         finally:
             sched.abort(rid)                         # gives back whatever is still held
 
+    def score(self, inputs: Sequence[int], top: int = 0) -> List[TokenLogprob]:
+        """What the model thinks of a given text: for every token behind the first, its log probability after those before it, the entropy there
+        and the `top` likeliest tokens.  With a `cache_budget` the text is read as a long prompt is, its cache cut between portions."""
+        tokens = self._check(inputs, 1, "score")
+        top = check_top(top, self.engine.spec.vocab_size, "score")
+        vocab = self.engine.spec.vocab_size
+        if min(tokens) < 0 or max(tokens) >= vocab:
+            raise ValueError(f"score: a token id is outside the vocabulary of {vocab}")
+        sched, engine, rid = Scheduler(self.engine, **self._sched_args), self.engine, object()
+        pending, given = [], torch.tensor(tokens[1:], dtype=torch.int32).to(engine.rt.device)
+        try:
+            for at in range(0, len(given), sched.chunk_size):
+                part = tokens[at:min(at + sched.chunk_size, len(given))]
+                logits = engine.step([StepEntry(rid, part, range(len(part)))])
+                pending.append(sched.sampler.logprobs_async(logits, given[at:at + len(part)], top))
+                sched.keep_within_budget([rid])
+            return [row for p in pending for row in p.result()]
+        finally:
+            engine.finish(rid)
+
     # ---- continuous batching ------------------------------------------------
     def engine_start(self) -> None:
         self._scheduler = Scheduler(self.engine, **self._sched_args)
@@ -134,10 +157,11 @@ class CausalLM:
         return self._scheduler
 
     def engine_add_request(self, inputs: Sequence[int], max_new_tokens: int = 128,
-                           sampling: Optional[SamplingParams] = None) -> int:
+                           sampling: Optional[SamplingParams] = None, logprobs: Optional[int] = None) -> int:
         """Returns the request id.  Without `sampling` the options given to
-        `engine_step` apply to the request, as in the reference."""
-        return self._sched().add_request(inputs, max_new_tokens, sampling)
+        `engine_step` apply to the request, as in the reference.  `logprobs`: the number of alternatives to keep beside
+        each generated token's log probability (`engine_get_logprobs`)."""
+        return self._sched().add_request(inputs, max_new_tokens, sampling, logprobs=logprobs)
 
     def engine_step(self, top_k: int = 1, top_p: float = 1.0, temperature: float = 1.0) -> int:
         """One step of continuous batching; returns how many requests finished in
@@ -160,6 +184,10 @@ class CausalLM:
 
     def engine_get_output(self, seq_id) -> List[int]:
         return self._sched().output(seq_id)
+
+    def engine_get_logprobs(self, seq_id) -> List[TokenLogprob]:
+        """One entry for every token of `engine_get_output`, of a request that was added with `logprobs`."""
+        return list(self._sched().requests[seq_id].logprobs)
 
     def engine_stop(self) -> None:
         if self._scheduler is not None:

@@ -8,6 +8,11 @@ query at position p sees keys t <= p, and with a window only p - t < window
 (src/ops/paged_attention/op.cpp:20-64); scale 1/sqrt(head_dim) unless given
 (:690 of qwen2.cpp); output projection (:699), added to the residual stream.
 The three projections are one product with a packed matrix [Wq; Wk; Wv].
+
+Where the runtime asks for it (`Runtime.attention_mass`), every cached key's row
+has a third tensor beside it: the attention weight that it has drawn from all
+queries so far, summed over the heads of its kv head, by which a cache of
+bounded length chooses what stays (`Engine.evict`).
 """
 from __future__ import annotations
 
@@ -17,7 +22,7 @@ import torch
 
 from ..kernels import ops
 from ..weights.loader import ParamSpec
-from .base import BatchNeeds, Mixer, PagedKVNeed, build_part, register_part
+from .base import BatchNeeds, Mixer, PagedKVNeed, PagedNeed, PagedTensor, build_part, register_part
 from .linear import Linear
 
 
@@ -48,7 +53,10 @@ class GQAttention(Mixer):
         return self.position is None or self.position.graph_safe
 
     def cache_need(self):
-        return PagedKVNeed(self.nkv, self.dh, self.window)
+        need = PagedKVNeed(self.nkv, self.dh, self.window)
+        if self.rt.attention_mass and not self.window:
+            need = PagedNeed(need.tensors + (PagedTensor("mass", (self.nkv, 1), torch.float32, accumulates=True),))
+        return need
 
     def batch_needs(self):
         # the kernels take single-token segments (split keys) and the others (tiles of queries) apart
@@ -114,6 +122,9 @@ class GQAttention(Mixer):
         attn = ctx.ws.buffer("attn.out", (qkv.shape[0], self.n_q), self.rt.dtype)
         ops.paged_attention(qkv, attn, cache.k, cache.v, ctx.attention_meta(cache.group),
                             self.nh, self.nkv, self.dh, cache.page_size, self.window, self.scale, ws=ctx.ws)
+        if "mass" in cache.tensors:
+            ops.attention_mass(qkv, cache.tensors["mass"], cache.k, ctx.attention_meta(cache.group), self.nh, self.nkv, self.dh,
+                               cache.page_size, self.scale, fresh=cache.owned, ws=ctx.ws)
         residual.add_linear(self.out, attn)
 
 

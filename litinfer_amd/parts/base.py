@@ -50,6 +50,8 @@ class Runtime:
     keep_stored_precision: bool = False
     # stored dtype -> number of matrices that were rounded to bfloat16 when they were bound
     rounded: Dict[str, int] = field(default_factory=dict, compare=False, hash=False)
+    # attention keeps, beside its keys, the weight that each has drawn so far (what `Engine.evict` goes by)
+    attention_mass: bool = False
     # tensor name -> the bound tensor, for a tensor that several parts read (one table cut into a slice a layer)
     shared: Dict[str, torch.Tensor] = field(default_factory=dict, compare=False, hash=False)
 
@@ -85,6 +87,8 @@ class PagedTensor:
     name: str
     shape: Tuple[int, ...]
     dtype: Optional[torch.dtype] = None
+    # a step adds to the rows of earlier tokens (the sums of attention weight): such a step cannot be taken back, nor a token run twice in it
+    accumulates: bool = False
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
         return (*self.shape[:-1], page_size, self.shape[-1])

@@ -1,3 +1,3 @@
-from .sampler import Sampler, SamplingParams, uniform
+from .sampler import PendingLogprobs, Sampler, SamplingParams, TokenLogprob, check_top, uniform
 
-__all__ = ["Sampler", "SamplingParams", "uniform"]
+__all__ = ["PendingLogprobs", "Sampler", "SamplingParams", "TokenLogprob", "check_top", "uniform"]

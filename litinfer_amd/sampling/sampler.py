@@ -22,9 +22,9 @@ import struct
 import threading
 from array import array
 from collections import deque
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from operator import attrgetter
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -136,6 +136,51 @@ class PendingTokens:
             self._sampler._give_back(self._host, self._event)
             self._host = self._event = None
         return self._tokens
+
+
+@dataclass(frozen=True)
+class TokenLogprob:
+    """What the model thought of one token: its log probability, the entropy of the distribution that it was taken from (nats), and the
+    likeliest tokens with theirs, in falling order."""
+    token: int
+    logprob: float
+    entropy: float
+    top: Tuple[Tuple[int, float], ...] = ()
+
+    def cut(self, top: int) -> "TokenLogprob":
+        return self if len(self.top) == top else replace(self, top=self.top[:top])
+
+
+def check_top(top, vocab: int, who: str) -> Optional[int]:
+    """The number of alternatives that a caller asks for, or None where it asks for no log probabilities."""
+    if top is None:
+        return None
+    if isinstance(top, bool) or not isinstance(top, (int, np.integer)) or not 0 <= top <= min(ops.LOGPROBS_MAX_TOP, vocab):
+        raise ValueError(f"{who}: the number of alternatives must lie between 0 and {min(ops.LOGPROBS_MAX_TOP, vocab)}, found {top!r}")
+    return int(top)
+
+
+class PendingLogprobs:
+    """Log probabilities that were worked out on the device and are on their way to the host."""
+
+    def __init__(self, sampler, host: torch.Tensor, n: int, top: int, event):
+        self._sampler, self._host, self._n, self._top, self._event = sampler, host, n, top, event
+        self._rows: Optional[List[TokenLogprob]] = None
+
+    def result(self) -> List[TokenLogprob]:
+        """One entry a row; waits for the device if they are not there yet."""
+        if self._rows is None:
+            if self._event is not None:
+                self._event.synchronize()
+            n, k, words = self._n, self._top, self._host
+            values = words.view(torch.float32)
+            ids, lp, ent = words[:n].tolist(), values[n:2 * n].tolist(), values[2 * n:3 * n].tolist()
+            top_ids = words[3 * n:3 * n + n * k].view(n, k).tolist()
+            top_lp = values[3 * n + n * k:3 * n + 2 * n * k].view(n, k).tolist()
+            self._rows = [TokenLogprob(t, a, b, tuple(zip(i, v))) for t, a, b, i, v in zip(ids, lp, ent, top_ids, top_lp)]
+            self._sampler._give_back(self._host, self._event)
+            self._host = self._event = None
+        return self._rows
 
 
 class Sampler:
@@ -269,6 +314,23 @@ class Sampler:
                 self._params_up = BatchUploader(self.device)       # pinned, so the copy does not wait for the stream
             ops.sample_rows_packed(logits, self._params_up.upload([host.view(np.int32)])[0], ids)
         return self._on_their_way(ids, n)
+
+    def logprobs_async(self, logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> PendingLogprobs:
+        """The log probability of token ids[i] (int32, on the device) in row i of logits [n, vocab], the row's entropy and its `top` likeliest
+        tokens, copied to the host without waiting."""
+        n, top = logits.shape[0], check_top(top, logits.shape[1], "logprobs")
+        words = torch.empty(n * (3 + 2 * top), dtype=torch.int32, device=logits.device)
+        values = words.view(torch.float32)
+        words[:n].copy_(ids)
+        top_ids = words[3 * n:3 * n + n * top].view(n, top) if top else None
+        top_lp = values[3 * n + n * top:].view(n, top) if top else None
+        ops.token_logprobs(logits, words[:n], values[n:2 * n], values[2 * n:3 * n], top_ids, top_lp)
+        host = self._host_buffer(words.numel())
+        event = None
+        host[:words.numel()].copy_(words, non_blocking=self.device.type == "cuda")
+        if self.device.type == "cuda":
+            event = self._record()
+        return PendingLogprobs(self, host, n, top, event)
 
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams],
                counters: Sequence[int]) -> List[int]:
