@@ -15,21 +15,47 @@
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// ------------------------------------------------------------------ attention weight, any head size
+// ------------------------------------------------------------------ attention weight
+// Two passes over the scores, since a weight needs the whole row's sum first: the rows' log-sums, then the columns' sums.  Scores
+// are held in powers of two (scale times log2 e); a row's statistic is lse = m + log2(sum of 2^(s - m)).
 struct MassArgs {
     const int *block_table, *q_start, *q_len, *ctx_len;
-    int max_blocks, nseg, nh, nkv, dh, page_size, num_pages, q_row_stride;
-    float scale;                 // times log2(e): scores are held in powers of two
+    int max_blocks, nh, nkv, dh, page_size, num_pages, q_row_stride;
+    uint32_t page_inv;           // 2^32 / page_size, rounded down (page_of)
+    float scale;                 // times log2(e)
     int fresh;                   // keys written by this step are set
 };
 
+// Segments of the batch that a launch takes, by value: a step's mix is known on the host, and what the workspace was laid out for is what the
+// kernels go by.  (A recorded step has single tokens only, all of them, and reads their contexts from the device.)
+#define EV_LIST 64
+struct SegList {
+    int n;                       // 0: segment i is the i-th, all of them, lengths from the device
+    int seg[EV_LIST], start[EV_LIST], q[EV_LIST], ctx[EV_LIST];
+    int off[EV_LIST];            // where the segment's places begin among all
+};
+
+// place / page_size and the rest: the product with the rounded-down inverse is at most one too small
+__device__ __forceinline__ int page_of(const MassArgs& a, int t, int& rest) {
+    int p = (int)__umulhi((uint32_t)t, a.page_inv);
+    rest = t - p * a.page_size;
+    if (rest >= a.page_size) { ++p; rest -= a.page_size; }
+    return p;
+}
 // place -> row of [kv heads, page size, *] inside the pool, or -1 where no page holds the place
-__device__ __forceinline__ long place_row(const MassArgs& a, int seg, int kvh, int t) {
-    const int page = a.block_table[(size_t)seg * a.max_blocks + t / a.page_size];
+__device__ __forceinline__ long place_row(const MassArgs& a, const int* table, int kvh, int t) {
+    int rest;
+    const int page = table[page_of(a, t, rest)];
     if (page < 0 || page >= a.num_pages) return -1;
-    return ((long)page * a.nkv + kvh) * a.page_size + t % a.page_size;
+    return ((long)page * a.nkv + kvh) * a.page_size + rest;
+}
+// the row of a place, some row where there is none (whoever asks does not use it)
+__device__ __forceinline__ long some_row(const MassArgs& a, const int* table, int kvh, int t) {
+    const long r = place_row(a, table, kvh, t);
+    return r < 0 ? (long)kvh * a.page_size : r;
 }
 
+// ---- any head size, type and alignment: scores by the vector ALU, computed twice
 template <typename T>
 __device__ __forceinline__ float dot_rows(const float* q, const T* k, int dh) {
     float s = 0.f;
@@ -37,18 +63,19 @@ __device__ __forceinline__ float dot_rows(const float* q, const T* k, int dh) {
     return s;
 }
 
-// lse [T, nh] (powers of two): a wave a (token, head), a key a lane.
+// lse [T, nh]: a wave a (token, head), a key a lane.
 template <typename T>
 __global__ __launch_bounds__(64) void mass_rows_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, float* __restrict__ lse) {
     __shared__ float qs[EV_MAX_DH];
     const int seg = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x;
     if (i >= a.q_len[seg]) return;
     const int tok = a.q_start[seg] + i, seen = a.ctx_len[seg] - a.q_len[seg] + i + 1;
+    const int* table = a.block_table + (size_t)seg * a.max_blocks;
     for (int d = lane; d < a.dh; d += 64) qs[d] = load_as_float(q + (size_t)tok * a.q_row_stride + (size_t)h * a.dh + d);
     __syncthreads();
     float m = -INFINITY, l = 0.f;
     for (int t = lane; t < seen; t += 64) {
-        const long row = place_row(a, seg, h / (a.nh / a.nkv), t);
+        const long row = place_row(a, table, h / (a.nh / a.nkv), t);
         if (row < 0) continue;
         const float s = dot_rows(qs, k + row * a.dh, a.dh) * a.scale;
         const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;     // (a score of NaN has no part in the maximum, but in the sum)
@@ -57,7 +84,8 @@ __global__ __launch_bounds__(64) void mass_rows_kernel(const T* __restrict__ q, 
     }
     const float mx = wave_max(m);
     l = wave_sum(m == -INFINITY ? l : l * exp2f(m - mx));
-    if (lane == 0) lse[(size_t)tok * a.nh + h] = l == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(l);     // (a row that sees nothing gives nothing)
+    // (a row that sees nothing gives nothing)
+    if (lane == 0) lse[(size_t)tok * a.nh + h] = l == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(l);
 }
 
 // A block takes 64 keys of a (request, kv head); its four waves take the queries in turn and are added up in their order.
@@ -68,11 +96,12 @@ __global__ __launch_bounds__(256) void mass_keys_kernel(const T* __restrict__ q,
     const int seg = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int nq = a.q_len[seg], ctx = a.ctx_len[seg], t = blockIdx.x * 64 + lane, rep = a.nh / a.nkv;
     if ((int)blockIdx.x * 64 >= ctx) return;
-    const long row = t < ctx ? place_row(a, seg, kvh, t) : -1;
+    const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
     const int base = ctx - nq;                           // place of the step's first token
     const int i0 = max((int)blockIdx.x * 64 - base, 0);  // the first query that sees any of the block's keys
     float sum = 0.f;
-    for (int i = i0; i < nq; i += 4)
+    for (int i = i0; i < nq; i += 4) {
+        float some = 0.f;                                // (a query's heads first: shorter sums keep their digits)
         for (int r = 0; r < rep; ++r) {
             const int mine = i + w, tok = a.q_start[seg] + mine, h = kvh * rep + r;
             __syncthreads();
@@ -80,8 +109,10 @@ __global__ __launch_bounds__(256) void mass_keys_kernel(const T* __restrict__ q,
                 for (int d = lane; d < a.dh; d += 64) qs[w][d] = load_as_float(q + (size_t)tok * a.q_row_stride + (size_t)h * a.dh + d);
             __syncthreads();
             if (mine < nq && row >= 0 && t <= base + mine)
-                sum += exp2f(dot_rows(qs[w], k + row * a.dh, a.dh) * a.scale - lse[(size_t)tok * a.nh + h]);
+                some += exp2f(dot_rows(qs[w], k + row * a.dh, a.dh) * a.scale - lse[(size_t)tok * a.nh + h]);
         }
+        sum += some;
+    }
     part[w][lane] = sum;
     __syncthreads();
     if (w || row < 0) return;
@@ -89,27 +120,599 @@ __global__ __launch_bounds__(256) void mass_keys_kernel(const T* __restrict__ q,
     mass[row] = a.fresh && t >= base ? sum : mass[row] + sum;
 }
 
-extern "C" long li_attention_mass_work_floats(int tokens, int nh) { return (long)tokens * nh; }
+// ---- on the matrix cores.  A lane's operand is a piece of 16 bytes of a row, as it lies in memory: 8 bfloat16 (one MFMA), or
+// 4 float32 (the e-th of four MFMAs takes the e-th; which k a slot stands for is the same on both sides).
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc, float* mass, int dtype, const int* block_table, int max_blocks,
-                                 const int* q_start, const int* q_len, const int* ctx_len, int nseg, int max_q_len, int max_ctx_len,
-                                 int nh, int nkv, int dh, int page_size, int num_pages, float scale, int fresh, float* work, hipStream_t stream) {
-    if (nseg <= 0 || nseg > 65535 || nh <= 0 || nh > 65535 || nkv <= 0 || nh % nkv || dh <= 0 || dh > EV_MAX_DH || page_size <= 0 || max_blocks <= 0 ||
-        max_q_len <= 0 || max_ctx_len < max_q_len || (long)max_ctx_len > (long)max_blocks * page_size || !work)
-        return LI_ERR_SIZE;
-    const MassArgs a = {block_table, q_start, q_len, ctx_len, max_blocks, nseg, nh, nkv, dh, page_size, num_pages, q_row_stride,
-                        scale * 1.44269504088896341f, fresh};
-    const dim3 rows(max_q_len, nh, nseg), keys((max_ctx_len + 63) / 64, nkv, nseg);
-    if (dtype == LI_F32) {
-        mass_rows_kernel<float><<<rows, 64, 0, stream>>>((const float*)q, (const float*)kc, a, work);
-        mass_keys_kernel<float><<<keys, 256, 0, stream>>>((const float*)q, (const float*)kc, a, work, mass);
-    } else if (dtype == LI_BF16) {
-        mass_rows_kernel<bf16_t><<<rows, 64, 0, stream>>>((const bf16_t*)q, (const bf16_t*)kc, a, work);
-        mass_keys_kernel<bf16_t><<<keys, 256, 0, stream>>>((const bf16_t*)q, (const bf16_t*)kc, a, work, mass);
+template <typename T>
+__device__ __forceinline__ f32x4_t mma16(const u32x4_t a, const u32x4_t b, f32x4_t c) {        // 16 x 16, rows of a against rows of b
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     } else {
-        return LI_ERR_DTYPE;
+        const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+}
+template <typename T>
+__device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x16_t c) {      // 32 x 32
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    } else {
+        const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// ---- single tokens.  The scores themselves are kept (4 bytes a query head and key beside the key's dh * 2): reading the keys
+// again would cost more.
+#define SG_KEYS 64                // keys of a wave
+#define SG_WAVES 4
+
+// Scores of 64 keys a wave against the heads of a kv head, 16 at a time, and the wave's maximum and sum for every head.
+// scores [request, nh, stride], stats [request, nh, parts] of (m, l).
+template <typename T, int CH>
+__global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
+                                                                           float* __restrict__ scores, long stride, float2* __restrict__ stats, int parts) {
+    constexpr int PE = 16 / sizeof(T);                   // elements of a piece
+    constexpr int NT = CH * 4 <= 16 ? 4 : CH * 2 <= 16 ? 2 : 1;      // tiles of 16 keys whose pieces are asked for at once
+    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int part = blockIdx.x * SG_WAVES + (threadIdx.x >> 6), k0 = part * SG_KEYS;
+    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS);
+    if (k0 >= ctx) return;
+    const int* table = a.block_table + (size_t)seg * a.max_blocks;
+    const int rep = a.nh / a.nkv, dh = a.dh;
+    long row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = k0 + 16 * i + c < ctx ? place_row(a, table, kvh, k0 + 16 * i + c) : -1;
+    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * dh;
+    const u32x4_t zero = {0, 0, 0, 0};
+    for (int h0 = 0; h0 < rep; h0 += 16) {
+        u32x4_t qf[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            const int d = (4 * j + g) * PE;
+            qf[j] = h0 + c < rep && d < dh ? *reinterpret_cast<const u32x4_t*>(qrow + (size_t)(h0 + c) * dh + d) : zero;
+        }
+        f32x4_t s[4];
+#pragma unroll
+        for (int i0 = 0; i0 < 4; i0 += NT) {
+            u32x4_t kf[NT][CH];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const int d = (4 * j + g) * PE;
+                    kf[i][j] = row[i0 + i] >= 0 && d < dh ? *reinterpret_cast<const u32x4_t*>(k + row[i0 + i] * dh + d) : zero;
+                }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < CH; ++j) acc = mma16<T>(kf[i][j], qf[j], acc);
+                s[i0 + i] = acc;
+            }
+        }
+        // lane (c, g) holds head c's scores of keys 16 i + 4 g + 0..3
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t there = (uint32_t)__ballot(row[i] >= 0) >> (4 * g);       // (lanes 0 .. 15: keys 16 i ..)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[i][r] = there >> r & 1 ? s[i][r] * a.scale : -INFINITY;
+                m = fmaxf(m, s[i][r]);
+            }
+        }
+        m = lane_xor_max(lane_xor_max(m, 16), 32);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(s[i][r] - base);
+        l = lane_xor_add(lane_xor_add(l, 16), 32);
+        if (h0 + c < rep) {
+            const size_t head = (size_t)req * a.nh + (size_t)kvh * rep + h0 + c;
+            float* out = scores + head * stride + k0 + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4_t*>(out + 16 * i) = s[i];      // (stride: whole runs of 64)
+            if (g == 0) stats[head * parts + part] = make_float2(m, l);
+        }
+    }
+}
+
+// lse of a head from the statistics of its `n` parts, by a wave.
+__device__ __forceinline__ float join_stats(const float2* st, int n, int lane) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 64) {
+        const float2 v = st[i];
+        const float mn = fmaxf(m, v.x), base = mn == -INFINITY ? 0.f : mn;
+        l = (m == -INFINITY ? l : l * exp2f(m - base)) + (v.x == -INFINITY ? v.y : v.y * exp2f(v.x - base));
+        m = mn;
+    }
+    const float mx = wave_max(m);
+    l = wave_sum(m == -INFINITY ? l : l * exp2f(m - mx));
+    return l == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(l);
+}
+
+#define SG_LSE 64                 // heads of a kv head whose lse a block holds at a time
+__global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegList list, const float* __restrict__ scores, long stride,
+                                                              const float2* __restrict__ stats, int parts, float* __restrict__ mass) {
+    __shared__ float lse[SG_LSE];
+    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS), t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
+    if ((int)blockIdx.x * 256 >= ctx) return;
+    const int n = (ctx + SG_KEYS - 1) / SG_KEYS;
+    const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
+    const float before = row >= 0 && !(a.fresh && t == ctx - 1) ? mass[row] : 0.f;
+    const size_t head0 = (size_t)req * a.nh + (size_t)kvh * rep;
+    float sum = 0.f;
+    for (int h0 = 0; h0 < rep; h0 += SG_LSE) {
+        const int heads = min(rep - h0, SG_LSE);
+        __syncthreads();
+        for (int h = w; h < heads; h += 4) {
+            const float v = join_stats(stats + (head0 + h0 + h) * parts, n, lane);
+            if (lane == 0) lse[h] = v;
+        }
+        __syncthreads();
+        if (row >= 0)
+            for (int h = 0; h < heads; ++h) sum += __builtin_amdgcn_exp2f(scores[(head0 + h0 + h) * stride + t] - lse[h]);
+    }
+    if (row >= 0) mass[row] = before + sum;
+}
+
+// ---- portions: tiles of 32 x 32 scores.  One side's rows stay in a wave's registers (ST tiles of 32 rows a wave), the other's go
+// through LDS, 64 rows a stage, two stages: loads go straight into LDS and fly while the stage before is multiplied.  A row's
+// pieces are swizzled (place p of row r holds piece p ^ (r & 7)), so that 8 rows' pieces of one column lie in different banks.
+#define PT_STAGE 64
+#define PT_WAVES 4
+
+// 16 bytes a lane from `src`, to `at` (an offset in LDS, the same in all lanes) + 16 * lane; nobody but s_waitcnt vmcnt knows when they have arrived.
+__device__ __forceinline__ void load_to_lds(const void* src, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+
+// All waves: rows r of the stage from row_ptr(r), `pieces` of 16 bytes a row, PPR places a row.
+template <int PPR, typename RowPtr>
+__device__ __forceinline__ void stage_rows(char* lds, int pieces, int w, int lane, RowPtr row_ptr) {
+    constexpr int LOADS = PT_STAGE * PPR / (64 * PT_WAVES);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int first = (w * LOADS + i) * 64, slot = first + lane, r = slot / PPR, p = (slot % PPR) ^ (r & 7);
+        if (p < pieces) {
+            load_to_lds(row_ptr(r) + 16 * p, lds_offset(lds) + 16 * first);
+        }
+    }
+}
+template <int PPR>
+__device__ __forceinline__ u32x4_t staged_piece(const char* lds, int r, int p) {
+    return *reinterpret_cast<const u32x4_t*>(lds + 16 * (r * PPR + (p ^ (r & 7))));
+}
+
+// Whether every place of 0 .. n - 1 has a page (the same answer in every thread of the block).
+__device__ __forceinline__ bool all_there(const MassArgs& a, const int* table, int n) {
+    const int blocks = (n + a.page_size - 1) / a.page_size;
+    int bad = 0;
+    for (int i = threadIdx.x; i < blocks; i += blockDim.x) bad |= table[i] < 0 || table[i] >= a.num_pages;
+    return !__syncthreads_or(bad);
+}
+
+// The rows' statistics: a wave holds ST * 32 queries of one head, the block streams keys.  Wave tiles of a kv head are numbered head
+// by head; a block takes four.  grid: x wave tiles / 4 (of the longest segment), y kv heads, z segments * splits of the keys.
+// stats [splits, T, nh].
+template <typename T, int DHP, int ST>
+__global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
+                                                                       float2* __restrict__ stats, int splits, int tokens) {
+    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, STAGE_BYTES = PT_STAGE * PPR * 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int which = blockIdx.z / splits, seg = list.seg[which], split = blockIdx.z % splits, kvh = blockIdx.y, tok0 = list.start[which];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
+    const int nq = list.q[which], base = list.ctx[which] - nq, rep = a.nh / a.nkv, pieces = a.dh / PE;
+    const int tiles = (nq + 32 * ST - 1) / (32 * ST), wt0 = blockIdx.x * PT_WAVES;
+    if (wt0 >= tiles * rep) return;
+    const int* table = a.block_table + (size_t)seg * a.max_blocks;
+    const int wt = min(wt0 + w, tiles * rep - 1);        // (a wave without a tile repeats the last one and stores nothing)
+    const bool mine = wt0 + w < tiles * rep;
+    const int h = kvh * rep + wt / tiles, i0 = wt % tiles * (32 * ST);
+    // the block's keys: up to the last that any of its waves sees, this split's share of the stages
+    int last = 0;
+    for (int i = 0; i < PT_WAVES; ++i) {
+        const int x = min(wt0 + i, tiles * rep - 1) % tiles * (32 * ST);
+        last = max(last, base + min(x + 32 * ST, nq) - 1);
+    }
+    const int stages = last / PT_STAGE + 1, s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
+    const bool whole = all_there(a, table, last + 1);
+    if (pieces < PPR) {
+        for (int i = tid; i < 2 * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
+    }
+    u32x4_t qf[ST][CH];
+    int pos[ST];
+#pragma unroll
+    for (int x = 0; x < ST; ++x) {
+        const int i = min(i0 + 32 * x + c, nq - 1);
+        pos[x] = base + i;
+        const T* src = q + (size_t)(tok0 + i) * a.q_row_stride + (size_t)h * a.dh;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) qf[x][j] = 2 * j + half < pieces ? *reinterpret_cast<const u32x4_t*>(src + (2 * j + half) * PE) : u32x4_t{0, 0, 0, 0};
+    }
+    const int seen_all = base + i0, seen_any = base + min(i0 + 32 * ST, nq) - 1;      // the wave's first and last query's places
+    float m[ST], l[ST];
+#pragma unroll
+    for (int x = 0; x < ST; ++x) { m[x] = -INFINITY; l[x] = 0.f; }
+    auto load = [&](int s, int buf) {
+        stage_rows<PPR>(lds + buf * STAGE_BYTES, pieces, w, lane, [&](int r) {
+            return (const char*)(k + some_row(a, table, kvh, min(s * PT_STAGE + r, last)) * a.dh);
+        });
+    };
+    if (s0 < s1) load(s0, 0);
+    for (int s = s0; s < s1; ++s) {
+        const int buf = (s - s0) & 1, k0 = s * PT_STAGE;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (s + 1 < s1) load(s + 1, buf ^ 1);
+        if (k0 > seen_any) continue;
+        const char* st = lds + buf * STAGE_BYTES;
+#pragma unroll
+        for (int y = 0; y < PT_STAGE / 32; ++y) {
+            f32x16_t acc[ST];
+#pragma unroll
+            for (int x = 0; x < ST; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const u32x4_t kf = staged_piece<PPR>(st, 32 * y + c, 2 * j + half);
+#pragma unroll
+                for (int x = 0; x < ST; ++x) acc[x] = mma32<T>(kf, qf[x][j], acc[x]);
+            }
+            // lane (c, half) holds query c's scores of keys 8 (r / 4) + 4 half + r % 4
+            const int t0 = k0 + 32 * y + 4 * half;
+            if (!whole || t0 - 4 * half + 31 > seen_all) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int t = t0 + 8 * (r >> 2) + (r & 3);
+                    const bool there = whole || (t <= last && place_row(a, table, kvh, t) >= 0);
+#pragma unroll
+                    for (int x = 0; x < ST; ++x) acc[x][r] = there && t <= pos[x] ? acc[x][r] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < ST; ++x) {
+                float mx = acc[x][0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, acc[x][r]);
+                const float mn = fmaxf(m[x], mx * a.scale), b = fmaxf(mn, -1e30f);       // (nothing seen yet: 2^(-inf + 1e30) is nothing)
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -b));
+                l[x] = l[x] * __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b) + sum;
+                m[x] = mn;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < ST; ++x) {
+        const float mx = lane_xor_max(m[x], 32), b = fmaxf(mx, -1e30f);
+        const float sum = lane_xor_add(l[x] * __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b), 32);
+        const int i = i0 + 32 * x + c;
+        if (mine && half == 0 && i < nq)
+            stats[((size_t)split * tokens + tok0 + i) * a.nh + h] = make_float2(mx, sum);
+    }
+}
+
+// lse [T, nh] from the splits' statistics (rows of other segments hold what they hold and are not asked for).
+__global__ __launch_bounds__(256) void mass_lse_kernel(const float2* __restrict__ stats, int splits, long rows, float* __restrict__ lse) {
+    const long i = blockIdx.x * 256L + threadIdx.x;
+    if (i >= rows) return;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const float2 v = stats[s * rows + i];
+        const float mn = fmaxf(m, v.x), b = fmaxf(mn, -1e30f);
+        l = l * exp2f(fmaxf(m, -1e30f) - b) + v.y * exp2f(fmaxf(v.x, -1e30f) - b);
+        m = mn;
+    }
+    lse[i] = l == 0.f ? INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+}
+
+// The columns' sums: a wave holds ST * 32 keys, the block streams the queries that see any of them, head by head.
+// grid: x blocks of keys (of the longest segment), y kv heads * splits of the (head, stage of queries) pairs, z segments.
+// part [splits, kv heads, places]; a segment's places begin at list.off.
+template <typename T, int DHP, int ST>
+__global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
+                                                                       const float* __restrict__ lse, float* __restrict__ part, int splits, long places) {
+    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, STAGE_BYTES = PT_STAGE * PPR * 16, KEYS = 32 * ST;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int which = blockIdx.z, seg = list.seg[which], kvh = blockIdx.y / splits, split = blockIdx.y % splits;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
+    const int nq = list.q[which], ctx = list.ctx[which], base = ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE, tok0 = list.start[which];
+    const int b0 = blockIdx.x * KEYS * PT_WAVES, k0 = b0 + w * KEYS;
+    if (b0 >= ctx) return;
+    const int* table = a.block_table + (size_t)seg * a.max_blocks;
+    if (pieces < PPR) {
+        for (int i = tid; i < 2 * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
+    }
+    u32x4_t kf[ST][CH];
+#pragma unroll
+    for (int x = 0; x < ST; ++x) {
+        const T* src = k + some_row(a, table, kvh, min(k0 + 32 * x + c, ctx - 1)) * a.dh;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) kf[x][j] = 2 * j + half < pieces ? *reinterpret_cast<const u32x4_t*>(src + (2 * j + half) * PE) : u32x4_t{0, 0, 0, 0};
+    }
+    float sums[ST][16];
+#pragma unroll
+    for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[x][r] = 0.f;
+    // pairs (head, stage of queries), numbered head by head; this split's share of them
+    const int first = max(b0 - base, 0) / PT_STAGE, n = (nq + PT_STAGE - 1) / PT_STAGE - first;
+    const int u0 = (int)((long)rep * n * split / splits), u1 = (int)((long)rep * n * (split + 1) / splits);
+    int lh = u0 / n, ls = first + u0 % n;                // the pair that is loaded next
+    auto load = [&](int buf) {
+        const T* src = q + (size_t)(kvh * rep + lh) * a.dh;
+        const int i0 = ls * PT_STAGE;
+        stage_rows<PPR>(lds + buf * STAGE_BYTES, pieces, w, lane, [&](int r) {
+            return (const char*)(src + (size_t)(tok0 + min(i0 + r, nq - 1)) * a.q_row_stride);
+        });
+    };
+    float lnext[PT_STAGE / 32];
+    auto load_lse = [&]() {
+#pragma unroll
+        for (int y = 0; y < PT_STAGE / 32; ++y) {
+            const int i = ls * PT_STAGE + 32 * y + c;
+            lnext[y] = i < nq ? lse[(size_t)(tok0 + i) * a.nh + kvh * rep + lh] : INFINITY;
+        }
+    };
+    auto advance = [&]() { if (++ls == first + n) { ls = first; ++lh; } };
+    int cs = ls;
+    if (u0 < u1) { load_lse(); load(0); advance(); }
+    for (int u = u0; u < u1; ++u) {
+        const int buf = (u - u0) & 1, i0 = cs * PT_STAGE;
+        float lq[PT_STAGE / 32];
+#pragma unroll
+        for (int y = 0; y < PT_STAGE / 32; ++y) lq[y] = lnext[y];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        cs = ls;
+        if (u + 1 < u1) { load_lse(); load(buf ^ 1); advance(); }
+        const char* st = lds + buf * STAGE_BYTES;
+#pragma unroll
+        for (int y = 0; y < PT_STAGE / 32; ++y) {
+            const int q0 = i0 + 32 * y;                  // the tile's first query
+            if (q0 >= nq || base + q0 + 31 < k0) continue;
+            f32x16_t acc[ST];
+#pragma unroll
+            for (int x = 0; x < ST; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const u32x4_t qf = staged_piece<PPR>(st, 32 * y + c, 2 * j + half);
+#pragma unroll
+                for (int x = 0; x < ST; ++x) acc[x] = mma32<T>(kf[x][j], qf, acc[x]);
+            }
+            if (base + q0 >= k0 + KEYS - 1) {            // every query sees every key
+#pragma unroll
+                for (int x = 0; x < ST; ++x)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums[x][r] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq[y]));
+            } else {
+                const int pos = base + q0 + c;
+#pragma unroll
+                for (int x = 0; x < ST; ++x)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq[y]));
+                        sums[x][r] += k0 + 32 * x + 4 * half + 8 * (r >> 2) + (r & 3) <= pos ? e : 0.f;
+                    }
+            }
+        }
+    }
+    float* out = part + ((size_t)split * a.nkv + kvh) * places + list.off[blockIdx.z];
+#pragma unroll
+    for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float v = sums[x][r];
+            v = lane_xor_add(lane_xor_add(lane_xor_add(lane_xor_add(lane_xor_add(v, 16), 8), 4), 2), 1);
+            const int t = k0 + 32 * x + 4 * half + 8 * (r >> 2) + (r & 3);
+            if (c == 0 && t < ctx) out[t] = v;
+        }
+}
+
+// The splits' sums, in their order, join the keys'.
+__global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list, const float* __restrict__ part, int splits, long places,
+                                                        float* __restrict__ mass) {
+    const int seg = list.seg[blockIdx.z], kvh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = list.ctx[blockIdx.z];
+    if (t >= ctx) return;
+    const long row = place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t);
+    if (row < 0) return;
+    const float* src = part + (size_t)kvh * places + list.off[blockIdx.z] + t;
+    float sum = 0.f;
+    for (int s = 0; s < splits; ++s) sum += src[(size_t)s * a.nkv * places];
+    mass[row] = a.fresh && t >= ctx - list.q[blockIdx.z] ? sum : mass[row] + sum;
+}
+
+// ---- the plan of a batch, from its segments in host memory: which kernels, how many splits, where things lie in the workspace
+struct MassPlan {
+    int single = 0, multi = 0;           // segments of one token, of more
+    int single_ctx = 0, multi_ctx = 0, multi_q = 0;
+    long stride = 0;                     // keys of a head's scores
+    int parts = 0;
+    int row_splits = 1, key_splits = 1, st = 1;
+    long places = 0;                     // of the longer segments' sums, all together
+    long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
+    bool tiled = false, valid = false;
+};
+
+struct Batch { const int *q_start, *q_len, *ctx_len; };      // in host memory
+
+static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, const void* k, float scale) {
+    const int es = dtype == LI_BF16 ? 2 : 4;
+    return dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
+}
+
+static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, bool f32, bool tiled) {
+    MassPlan p;
+    long total = 0, pairs = 0;
+    const int keys = 32 * PT_WAVES * (f32 ? 1 : 2);
+    for (int i = 0; i < nseg; ++i) {
+        const int ctx = padded_ctx > 0 ? padded_ctx : ctx_len[i];
+        if (q_len[i] <= 0 || ctx < q_len[i]) return p;
+        total += q_len[i];
+        if (q_len[i] == 1 && tiled) {
+            ++p.single;
+            p.single_ctx = ctx > p.single_ctx ? ctx : p.single_ctx;
+        } else {
+            ++p.multi;
+            p.multi_ctx = ctx > p.multi_ctx ? ctx : p.multi_ctx;
+            p.multi_q = q_len[i] > p.multi_q ? q_len[i] : p.multi_q;
+            p.places += (ctx + keys - 1) / keys * (long)keys;
+            pairs += (ctx + keys - 1) / keys;
+        }
+    }
+    if (total != tokens || p.places >= 1L << 31) return p;
+    p.valid = true;
+    p.tiled = tiled;
+    const int rep = nh / nkv;
+    if (!tiled) { p.floats = (long)tokens * nh; return p; }
+    if (p.single) {
+        p.parts = (p.single_ctx + SG_KEYS - 1) / SG_KEYS;
+        p.stride = (long)p.parts * SG_KEYS;
+        p.scores = 0;
+        p.stats = (long)p.single * nh * p.stride;
+        p.floats = p.stats + 2L * p.single * nh * p.parts;
+    }
+    if (p.multi) {
+        p.st = f32 ? 1 : 2;
+        const long row_blocks = ((long)(p.multi_q + 32 * p.st - 1) / (32 * p.st) * rep + PT_WAVES - 1) / PT_WAVES * nkv * p.multi;
+        const int stages = (p.multi_ctx + PT_STAGE - 1) / PT_STAGE;
+        while (p.row_splits < 16 && row_blocks * p.row_splits < 512 && stages / (2 * p.row_splits) >= 4) p.row_splits *= 2;
+        const long key_blocks = pairs * nkv, units = (long)rep * ((p.multi_q + PT_STAGE - 1) / PT_STAGE);
+        while (p.key_splits < 16 && key_blocks * p.key_splits < 1024 && units / (2 * p.key_splits) >= 2) p.key_splits *= 2;
+        p.rows = p.floats;
+        p.lse = p.rows + 2L * p.row_splits * tokens * nh;
+        p.sums = p.lse + (long)tokens * nh;
+        p.floats = p.sums + (long)p.key_splits * nkv * p.places;
+    }
+    return p;
+}
+
+// Floats of workspace for a batch (its segments in host memory); -1: not a batch.  padded_ctx > 0: a batch that is recorded and replayed
+// for any contexts up to that.  q, k: the addresses, whose alignment decides on the kernel.
+extern "C" long li_attention_mass_work_floats(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, int dtype,
+                                              int q_row_stride, const void* q, const void* k, float scale) {
+    if (nseg <= 0 || tokens <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || !q_len || !ctx_len) return -1;
+    const MassPlan p = mass_plan(q_len, ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, k, scale));
+    return p.valid ? p.floats : -1;
+}
+
+template <typename K>
+static bool allow_lds(K kernel, int bytes) {
+    return bytes <= 64 * 1024 || hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+}
+
+template <typename T, int DHP>
+static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg,
+                             int tokens, float* work, hipStream_t stream) {
+    constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1, KEYS = 32 * ST * PT_WAVES;
+    constexpr int LDS_BYTES = 2 * PT_STAGE * DHP * (int)sizeof(T);
+    if (p.single) {
+        for (int at = 0, i = 0; at < p.single;) {
+            SegList list;
+            list.n = 0;
+            int n = p.single;
+            if (p.single < nseg) {                       // a mix: the single ones are named
+                n = 0;
+                for (; i < nseg && n < EV_LIST; ++i)
+                    if (b.q_len[i] == 1) {
+                        list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = 1; list.ctx[n] = b.ctx_len[i]; list.off[n++] = 0;
+                    }
+                list.n = n;
+            }
+            float* scores = work + p.scores + (size_t)at * a.nh * p.stride;
+            float2* stats = (float2*)(work + p.stats) + (size_t)at * a.nh * p.parts;
+            mass_single_scores_kernel<T, CH16><<<dim3((p.parts + SG_WAVES - 1) / SG_WAVES, a.nkv, n), 64 * SG_WAVES, 0, stream>>>(
+                q, k, a, list, scores, p.stride, stats, p.parts);
+            mass_single_add_kernel<<<dim3((p.single_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, scores, p.stride, stats, p.parts, mass);
+            at += n;
+        }
+    }
+    if (p.multi) {
+        const auto rows = mass_rows_tile_kernel<T, DHP, ST>;
+        const auto keys = mass_keys_tile_kernel<T, DHP, ST>;
+        if (!allow_lds(rows, LDS_BYTES) || !allow_lds(keys, LDS_BYTES)) return LI_ERR_LAUNCH;
+        const int rep = a.nh / a.nkv, tiles = (p.multi_q + 32 * ST - 1) / (32 * ST);
+        float2* stats = (float2*)(work + p.rows);
+        float *lse = work + p.lse, *sums = work + p.sums;
+        const long rows_n = (long)tokens * a.nh;
+        for (int pass = 0; pass < 2; ++pass) {
+            long off = 0;
+            for (int at = 0, i = 0; at < p.multi;) {
+                SegList list;
+                int n = 0;
+                for (; i < nseg && n < EV_LIST; ++i)
+                    if (b.q_len[i] > 1) {
+                        list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = b.q_len[i]; list.ctx[n] = b.ctx_len[i]; list.off[n++] = (int)off;
+                        off += (b.ctx_len[i] + KEYS - 1) / KEYS * (long)KEYS;
+                    }
+                list.n = n;
+                at += n;
+                if (pass == 0) {
+                    rows<<<dim3((tiles * rep + PT_WAVES - 1) / PT_WAVES, a.nkv, n * p.row_splits), 64 * PT_WAVES, LDS_BYTES, stream>>>(
+                        q, k, a, list, stats, p.row_splits, tokens);
+                } else {
+                    keys<<<dim3((p.multi_ctx + KEYS - 1) / KEYS, a.nkv * p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
+                        q, k, a, list, lse, sums, p.key_splits, p.places);
+                    mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, p.key_splits, p.places, mass);
+                }
+            }
+            if (pass == 0) mass_lse_kernel<<<(unsigned)((rows_n + 255) / 256), 256, 0, stream>>>(stats, p.row_splits, rows_n, lse);
+        }
     }
     return li_launch_status();
+}
+
+template <typename T>
+static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg, int tokens,
+                       float* work, hipStream_t stream) {
+    if (p.tiled && a.dh <= 64) return launch_mass_tiled<T, 64>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    if (p.tiled && a.dh <= 128) return launch_mass_tiled<T, 128>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    if (p.tiled) return launch_mass_tiled<T, 256>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    mass_rows_kernel<T><<<dim3(p.multi_q, a.nh, nseg), 64, 0, stream>>>(q, k, a, work);
+    mass_keys_kernel<T><<<dim3((p.multi_ctx + 63) / 64, a.nkv, nseg), 256, 0, stream>>>(q, k, a, work, mass);
+    return li_launch_status();
+}
+
+// q_start, q_len, ctx_len: the batch's segments on the device; those with h_ the same in host memory.  padded_ctx > 0: the contexts may be others
+// when a recording is replayed, up to that; then every segment brings one token.  work: li_attention_mass_work_floats of the same batch.
+extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc, float* mass, int dtype, const int* block_table, int max_blocks,
+                                 const int* q_start, const int* q_len, const int* ctx_len, const int* h_q_start, const int* h_q_len,
+                                 const int* h_ctx_len, int nseg, int tokens,
+                                 int padded_ctx, int nh, int nkv, int dh, int page_size, int num_pages, float scale, int fresh, float* work,
+                                 hipStream_t stream) {
+    if (nseg <= 0 || nseg > 65535 || tokens <= 0 || nh <= 0 || nh > 65535 || nkv <= 0 || nkv > 4095 || nh % nkv || dh <= 0 || dh > EV_MAX_DH || page_size <= 0 ||
+        max_blocks <= 0 || (long)max_blocks * page_size >= 1L << 31 || num_pages <= 0 || !h_q_start || !h_q_len || !h_ctx_len || !work)
+        return LI_ERR_SIZE;
+    const long room = (long)max_blocks * page_size;
+    for (int i = 0; i < nseg; ++i)
+        if (h_ctx_len[i] > room || h_q_start[i] < 0 || (long)h_q_start[i] + h_q_len[i] > tokens || (padded_ctx > 0 && (h_q_len[i] != 1 || padded_ctx > room))) return LI_ERR_SIZE;
+    if (dtype != LI_F32 && dtype != LI_BF16) return LI_ERR_DTYPE;
+    const MassArgs a = {block_table, q_start, q_len, ctx_len, max_blocks, nh, nkv, dh, page_size, num_pages, q_row_stride,
+                        (uint32_t)(page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size)), scale * 1.44269504088896341f, fresh};
+    const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale));
+    if (!p.valid) return LI_ERR_SIZE;
+    const Batch b = {h_q_start, h_q_len, h_ctx_len};
+    if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, nseg, tokens, work, stream);
+    return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, nseg, tokens, work, stream);
 }
 
 // ------------------------------------------------------------------ which keys stay

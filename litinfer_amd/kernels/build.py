@@ -33,6 +33,8 @@ FLAGS = ["-O3", "-std=c++17", "-shared", "-fPIC", f"--offload-arch={ARCH}",
 # with the accumulators in ordinary vector registers this needs no copies to and from the
 # accumulation registers (and fewer registers in all).
 MODULE_FLAGS = {"attention": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                # (as attention; and loads into LDS as in the products)
+                "evict": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Wno-inline-asm"],
                 # the products' loads into LDS are inline assembly that sets M0 and says so in its clobber
                 # list, which the compiler remarks upon for every instance
                 "gemm": ["-Wno-inline-asm"], "moe": ["-Wno-inline-asm"]}

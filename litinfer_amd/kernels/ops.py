@@ -118,7 +118,7 @@ _SIGNATURES = {
         "li_token_logprobs": [P, L, P, I, I, I, P, P, P, P, P],
     },
     "evict": {
-        "li_attention_mass": [P, I, P, P, I, P, I, P, P, P, I, I, I, I, I, I, I, I, F, I, P],
+        "li_attention_mass": [P, I, P, P, I, P, I, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P],
         "li_evict_select": [P, P, I, P, P, I, I, I, P, I, I, I, I, I],
         "li_cache_compact": [P, P, I, P, I, P, I, I, I, I, I, I],
     },
@@ -2004,13 +2004,22 @@ def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta,
     _chk(meta.max_blocks * page_size >= meta.max_ctx_len, "attention_mass: block table too short")
     if not t:
         return
+    hs, hq, hc = meta.host_q_start, meta.host_q_len, meta.host_ctx_len
+    _chk(all(isinstance(x, np.ndarray) and x.dtype == np.int32 and x.shape == (n,) and x.flags.c_contiguous for x in (hs, hq, hc)),
+         "attention_mass: host_q_start, host_q_len and host_ctx_len must be int32 [segments]")
     # (a recorded step is replayed for longer contexts of the same tables)
-    keys = meta.max_blocks * page_size if meta.padded else meta.max_ctx_len
-    need = int(_lib_fn("evict", "li_attention_mass_work_floats", [c_int, c_int], c_long)(t, nh))
+    padded = meta.max_blocks * page_size if meta.padded else 0
+    dt, hq, hc = _DT[qkv.dtype], hq.ctypes.data, hc.ctypes.data
+    need = _mass_work_floats()(hq, hc, n, t, padded, nh, nkv, dh, dt, qkv.stride(0), qkv.data_ptr(), k.data_ptr(), float(scale))
+    _chk(need >= 0, "attention_mass: the segments' lengths are not those of a batch")
     work = ws.buffer("evict.mass", (need,), torch.float32) if ws is not None else _scratch.floats(need, qkv.device)
-    _run("evict", "li_attention_mass", qkv.data_ptr(), qkv.stride(0), k.data_ptr(), mass.data_ptr(), _DT[qkv.dtype], bt.data_ptr(), meta.max_blocks,
-         meta.q_start.data_ptr(), meta.q_len.data_ptr(), meta.ctx_len.data_ptr(), n, meta.max_q_len, keys, nh, nkv, dh, page_size, k.shape[0],
-         float(scale), int(bool(fresh)), work.data_ptr())
+    _run("evict", "li_attention_mass", qkv.data_ptr(), qkv.stride(0), k.data_ptr(), mass.data_ptr(), dt, bt.data_ptr(), meta.max_blocks,
+         meta.q_start.data_ptr(), meta.q_len.data_ptr(), meta.ctx_len.data_ptr(), hs.ctypes.data, hq, hc, n, t, padded, nh, nkv, dh, page_size,
+         k.shape[0], float(scale), int(bool(fresh)), work.data_ptr())
+
+
+def _mass_work_floats():
+    return _lib_fn("evict", "li_attention_mass_work_floats", [P, P] + [I] * 8 + [P, P, F], c_long)
 
 
 def _check_requests(what: str, block_table, n: int, page_size: int) -> None:
