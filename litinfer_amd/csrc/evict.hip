@@ -11,6 +11,8 @@
 // place / page size to the page.
 #include "common.h"
 
+#include <type_traits>
+
 #define EV_MAX_DH 256
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -268,10 +270,17 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
 }
 
 // ---- portions: tiles of 32 x 32 scores.  One side's rows stay in a wave's registers (ST tiles of 32 rows a wave), the other's go
-// through LDS, 64 rows a stage, two stages: loads go straight into LDS and fly while the stage before is multiplied.  A row's
-// pieces are swizzled (place p of row r holds piece p ^ (r & 7)), so that 8 rows' pieces of one column lie in different banks.
-#define PT_STAGE 64
+// through LDS in stages of 64 rows (32 where three of 64 do not fit).  Loads go straight into LDS; a stage is asked for while the one before
+// the last is worked on.  A row's pieces are swizzled (place p of row r holds piece p ^ (r & 15)), so that rows' pieces of one column lie
+// in different banks.
+//
+// A step is one tile of 32 staged rows: its products, beside them the exponentials of the tile before (MFMAs and the vector ALU work side by
+// side), and the first pieces of the next tile's rows, which then wait in registers.  What bounds a step is the exponentials and sums:
+// 96 vector instructions against 16 MFMAs.
 #define PT_WAVES 4
+#define PT_BUFS 3
+#define PT_RING 4                 // pieces of a row that are read ahead
+constexpr int stage_tiles(int row_bytes) { return PT_BUFS * 64 * row_bytes <= 159 * 1024 ? 2 : 1; }
 
 // 16 bytes a lane from `src`, to `at` (an offset in LDS, the same in all lanes) + 16 * lane; nobody but s_waitcnt vmcnt knows when they have arrived.
 __device__ __forceinline__ void load_to_lds(const void* src, uint32_t at) {
@@ -279,21 +288,69 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint32_t at) {
 }
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 
-// All waves: rows r of the stage from row_ptr(r), `pieces` of 16 bytes a row, PPR places a row.
-template <int PPR, typename RowPtr>
-__device__ __forceinline__ void stage_rows(char* lds, int pieces, int w, int lane, RowPtr row_ptr) {
-    constexpr int LOADS = PT_STAGE * PPR / (64 * PT_WAVES);
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int first = (w * LOADS + i) * 64, slot = first + lane, r = slot / PPR, p = (slot % PPR) ^ (r & 7);
-        if (p < pieces) {
-            load_to_lds(row_ptr(r) + 16 * p, lds_offset(lds) + 16 * first);
-        }
-    }
+// The wave's loads but the `LATER` youngest have arrived, and with them, behind the barrier, all waves' (a wave's loads retire in order).
+template <int LATER>
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+    __syncthreads();
 }
 template <int PPR>
-__device__ __forceinline__ u32x4_t staged_piece(const char* lds, int r, int p) {
-    return *reinterpret_cast<const u32x4_t*>(lds + 16 * (r * PPR + (p ^ (r & 7))));
+__device__ __forceinline__ int swizzle(int r) { return r & (PPR < 16 ? PPR - 1 : 15); }
+
+// All waves: ROWS rows, row r from the piece row_at(r) of src on, `pieces` of 16 bytes a row, PPR places a row.
+template <int PPR, int ROWS, typename RowAt>
+__device__ __forceinline__ void stage_rows(char* lds, const void* src, int pieces, int w, int lane, RowAt row_at) {
+    constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int first = (w * LOADS + i) * 64, slot = first + lane, r = slot / PPR, p = (slot % PPR) ^ swizzle<PPR>(r);
+        const uint32_t piece = row_at(r) + p;
+        if (p < pieces) load_to_lds((const u32x4_t*)src + piece, lds_offset(lds) + 16 * first);
+    }
+}
+// Where a lane's pieces of its row lie in a tile.
+template <int PPR>
+__device__ __forceinline__ void staged_at(int c, int half, int (&at)[PPR / 2]) {
+#pragma unroll
+    for (int j = 0; j < PPR / 2; ++j) at[j] = 16 * (c * PPR + ((2 * j + half) ^ swizzle<PPR>(c)));
+}
+__device__ __forceinline__ u32x4_t staged_piece(const char* rows, int at) { return *reinterpret_cast<const u32x4_t*>(rows + at); }
+
+// The tile `rows` against the ST tiles that are held.  ring holds the tile's first pieces; each that has been used makes room for the piece
+// PT_RING further on, behind the last for the first ones of the tile `next`.  beside(j) is the share of other work between piece j's
+// products and the next's: the order is kept as it is written.
+template <int CH, int ST, typename Mma, typename Beside>
+__device__ __forceinline__ void multiply_rows(const char* rows, const char* next, const int (&at)[CH], u32x4_t (&ring)[PT_RING], const u32x4_t (&held)[ST][CH],
+                                              f32x16_t (&acc)[ST], Mma mma, Beside beside) {
+    const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    static_assert(CH % PT_RING == 0, "a tile begins at the ring's beginning");
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+#pragma unroll
+        for (int x = 0; x < ST; ++x) acc[x] = mma(ring[j % PT_RING], held[x][j], j ? acc[x] : zero);
+        ring[j % PT_RING] = j + PT_RING < CH ? staged_piece(rows, at[j + PT_RING]) : staged_piece(next, at[j + PT_RING - CH]);
+        beside(j);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+template <int ST>
+__device__ __forceinline__ void nothing(f32x16_t (&acc)[ST]) {
+#pragma unroll
+    for (int x = 0; x < ST; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[x][r] = -INFINITY;
+}
+// Calls step(constant i, t) for t = 0 .. n - 1 with i = t modulo 6: buffers, tiles of a stage and accumulators are constants of the code.
+template <typename Step>
+__device__ __forceinline__ void in_steps(int n, Step step) {
+    for (int t = 0; t < n; t += 6) {
+        step(std::integral_constant<int, 0>{}, t);
+        if (t + 1 < n) step(std::integral_constant<int, 1>{}, t + 1);
+        if (t + 2 < n) step(std::integral_constant<int, 2>{}, t + 2);
+        if (t + 3 < n) step(std::integral_constant<int, 3>{}, t + 3);
+        if (t + 4 < n) step(std::integral_constant<int, 4>{}, t + 4);
+        if (t + 5 < n) step(std::integral_constant<int, 5>{}, t + 5);
+    }
 }
 
 // Whether every place of 0 .. n - 1 has a page (the same answer in every thread of the block).
@@ -304,33 +361,30 @@ __device__ __forceinline__ bool all_there(const MassArgs& a, const int* table, i
     return !__syncthreads_or(bad);
 }
 
-// The rows' statistics: a wave holds ST * 32 queries of one head, the block streams keys.  Wave tiles of a kv head are numbered head
-// by head; a block takes four.  grid: x wave tiles / 4 (of the longest segment), y kv heads, z segments * splits of the keys.
-// stats [splits, T, nh].
+// The rows' statistics: a wave holds ST * 32 queries of one head, the block streams keys.  Wave tiles of a kv head are numbered from the
+// last queries, whose rows are the longest, to the first, a tile's heads side by side: the four that a block takes see about the same keys.  grid: x kv heads times wave tiles / 4 (of the longest segment), z segments * splits of the keys.  The kv head
+// goes fastest, here and below: blocks go round the XCDs, so an XCD's second-level cache holds one kv head's rows, or a few.
+// stats [splits, T, nh], or, where there is one split, lse [T, nh] itself.
 template <typename T, int DHP, int ST>
 __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                       float2* __restrict__ stats, int splits, int tokens) {
-    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, STAGE_BYTES = PT_STAGE * PPR * 16;
+                                                                       float2* __restrict__ stats, float* __restrict__ lse, int splits, int tokens) {
+    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int which = blockIdx.z / splits, seg = list.seg[which], split = blockIdx.z % splits, kvh = blockIdx.y, tok0 = list.start[which];
+    const int which = blockIdx.z / splits, seg = list.seg[which], split = blockIdx.z % splits, kvh = blockIdx.x % a.nkv, tok0 = list.start[which];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
     const int nq = list.q[which], base = list.ctx[which] - nq, rep = a.nh / a.nkv, pieces = a.dh / PE;
-    const int tiles = (nq + 32 * ST - 1) / (32 * ST), wt0 = blockIdx.x * PT_WAVES;
+    const int tiles = (nq + 32 * ST - 1) / (32 * ST), wt0 = blockIdx.x / a.nkv * PT_WAVES;
     if (wt0 >= tiles * rep) return;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
     const int wt = min(wt0 + w, tiles * rep - 1);        // (a wave without a tile repeats the last one and stores nothing)
     const bool mine = wt0 + w < tiles * rep;
-    const int h = kvh * rep + wt / tiles, i0 = wt % tiles * (32 * ST);
-    // the block's keys: up to the last that any of its waves sees, this split's share of the stages
-    int last = 0;
-    for (int i = 0; i < PT_WAVES; ++i) {
-        const int x = min(wt0 + i, tiles * rep - 1) % tiles * (32 * ST);
-        last = max(last, base + min(x + 32 * ST, nq) - 1);
-    }
-    const int stages = last / PT_STAGE + 1, s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
+    const int h = kvh * rep + wt % rep, i0 = (tiles - 1 - wt / rep) * (32 * ST);
+    // the block's keys: up to the last that its first wave sees, this split's share of the stages
+    const int last = base + min((tiles - wt0 / rep) * (32 * ST), nq) - 1;
+    const int stages = last / ROWS + 1, s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
     const bool whole = all_there(a, table, last + 1);
     if (pieces < PPR) {
-        for (int i = tid; i < 2 * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
+        for (int i = tid; i < PT_BUFS * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
         __syncthreads();
     }
     u32x4_t qf[ST][CH];
@@ -347,64 +401,103 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     float m[ST], l[ST];
 #pragma unroll
     for (int x = 0; x < ST; ++x) { m[x] = -INFINITY; l[x] = 0.f; }
-    auto load = [&](int s, int buf) {
-        stage_rows<PPR>(lds + buf * STAGE_BYTES, pieces, w, lane, [&](int r) {
-            return (const char*)(k + some_row(a, table, kvh, min(s * PT_STAGE + r, last)) * a.dh);
-        });
+    // (the rows of a stage are looked up in the table a stage before they are asked for, one a lane)
+    constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
+    int row = 0;
+    auto look_up = [&](int s) __attribute__((always_inline)) { row = (int)some_row(a, table, kvh, min(s * ROWS + lane % ROWS, last)) * pieces; };
+    auto load = [&](int buf) __attribute__((always_inline)) {
+        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, k, pieces, w, lane, [&](int r) { return (uint32_t)__shfl(row, r, LI_WAVE); });
     };
-    if (s0 < s1) load(s0, 0);
-    for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1, k0 = s * PT_STAGE;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (s + 1 < s1) load(s + 1, buf ^ 1);
-        if (k0 > seen_any) continue;
-        const char* st = lds + buf * STAGE_BYTES;
+    int at[CH];
+    staged_at<PPR>(c, half, at);
+    u32x4_t ring[PT_RING];
+    // lane (c, half) gets query c's scores of keys 8 (r / 4) + 4 half + r % 4
+    // A tile joins the rows' statistics in CH shares: the first quarter finds the maxima, the others add up.
+    float b[ST], sum[ST];
+    constexpr int LEAD = CH / 4, EACH = CH - LEAD;
+    auto share = [&](const f32x16_t (&acc)[ST], int j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int y = 0; y < PT_STAGE / 32; ++y) {
-            f32x16_t acc[ST];
-#pragma unroll
-            for (int x = 0; x < ST; ++x)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const u32x4_t kf = staged_piece<PPR>(st, 32 * y + c, 2 * j + half);
-#pragma unroll
-                for (int x = 0; x < ST; ++x) acc[x] = mma32<T>(kf, qf[x][j], acc[x]);
-            }
-            // lane (c, half) holds query c's scores of keys 8 (r / 4) + 4 half + r % 4
-            const int t0 = k0 + 32 * y + 4 * half;
-            if (!whole || t0 - 4 * half + 31 > seen_all) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int t = t0 + 8 * (r >> 2) + (r & 3);
-                    const bool there = whole || (t <= last && place_row(a, table, kvh, t) >= 0);
-#pragma unroll
-                    for (int x = 0; x < ST; ++x) acc[x][r] = there && t <= pos[x] ? acc[x][r] : -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < ST; ++x) {
+        for (int x = 0; x < ST; ++x) {
+            if (j == x * LEAD / ST) {
                 float mx = acc[x][0];
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = fmaxf(mx, acc[x][r]);
-                const float mn = fmaxf(m[x], mx * a.scale), b = fmaxf(mn, -1e30f);       // (nothing seen yet: 2^(-inf + 1e30) is nothing)
-                float sum = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -b));
-                l[x] = l[x] * __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b) + sum;
+                const float mn = fmaxf(m[x], mx * a.scale);
+                b[x] = fmaxf(mn, -1e30f);                // (nothing seen yet: 2^(-inf + 1e30) is nothing)
+                l[x] *= __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b[x]);
                 m[x] = mn;
+                sum[x] = 0.f;
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (j >= LEAD && (16 * x + r) * EACH / (16 * ST) == j - LEAD) sum[x] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -b[x]));
+            if (j == CH - 1) l[x] += sum[x];
         }
+    };
+    // keys that a query does not see, if there may be any among these 32
+    auto hide = [&](f32x16_t (&acc)[ST], int k0) __attribute__((always_inline)) {
+        if (whole && k0 + 31 <= seen_all) return;
+        uint32_t there = ~0u;
+        if (!whole) there = (uint32_t)__ballot(place_row(a, table, kvh, min(k0 + c, last)) >= 0);
+        there >>= 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = 8 * (r >> 2) + (r & 3);
+#pragma unroll
+            for (int x = 0; x < ST; ++x) acc[x][r] = (there >> i & 1) && k0 + 4 * half + i <= pos[x] ? acc[x][r] : -INFINITY;
+        }
+    };
+    auto stay = [&]() __attribute__((always_inline)) {   // (the compiler would move the exponentials behind the branch that follows)
+#pragma unroll
+        for (int x = 0; x < ST; ++x) asm volatile("" : "+v"(m[x]), "+v"(l[x]));
+    };
+    f32x16_t acc[2][ST];
+    nothing<ST>(acc[0]);
+    nothing<ST>(acc[1]);
+    int pending = 0;
+    if (s0 < s1) {
+        look_up(s0);
+        load(0);
+        look_up(s0 + 1);
+        if (s0 + 1 < s1) {
+            load(1);
+            look_up(s0 + 2);
+            arrived<LOADS>();
+        } else {
+            arrived<0>();
+        }
+#pragma unroll
+        for (int j = 0; j < PT_RING; ++j) ring[j] = staged_piece(lds, at[j]);
+    }
+    in_steps((s1 - s0) * TPS, [&](auto index, int t) __attribute__((always_inline)) {
+        constexpr int I = decltype(index)::value, buf = I / TPS % PT_BUFS, y = I % TPS, nbuf = (I + 1) / TPS % PT_BUFS, ny = (I + 1) % TPS, now = I & 1;
+        const int s = s0 + t / TPS, k0 = s * ROWS + 32 * y;
+        if (y == TPS - 1 && s + 1 < s1) {                // the next stage is there, and nobody reads the one before this any more
+            arrived<0>();
+            if (s + 2 < s1) { load((buf + 2) % PT_BUFS); look_up(s + 3); }
+        }
+        if (k0 > seen_any) return;
+        multiply_rows<CH, ST>(lds + buf * STAGE_BYTES + 32 * y * PPR * 16, lds + nbuf * STAGE_BYTES + 32 * ny * PPR * 16, at, ring, qf, acc[now],
+                              [](const u32x4_t staged, const u32x4_t held, f32x16_t v) { return mma32<T>(staged, held, v); },
+                              [&](int j) __attribute__((always_inline)) { share(acc[now ^ 1], j); });
+        stay();
+        hide(acc[now], k0);
+        pending = now;
+    });
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {                       // the last tile's
+        if (pending == 0) share(acc[0], j);
+        else share(acc[1], j);
     }
 #pragma unroll
     for (int x = 0; x < ST; ++x) {
         const float mx = lane_xor_max(m[x], 32), b = fmaxf(mx, -1e30f);
         const float sum = lane_xor_add(l[x] * __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b), 32);
         const int i = i0 + 32 * x + c;
-        if (mine && half == 0 && i < nq)
-            stats[((size_t)split * tokens + tok0 + i) * a.nh + h] = make_float2(mx, sum);
+        if (!mine || half != 0 || i >= nq) continue;
+        const size_t at = (size_t)(tok0 + i) * a.nh + h;
+        if (splits > 1) stats[(size_t)split * tokens * a.nh + at] = make_float2(mx, sum);
+        else lse[at] = sum == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(sum);
     }
 }
 
@@ -423,21 +516,22 @@ __global__ __launch_bounds__(256) void mass_lse_kernel(const float2* __restrict_
 }
 
 // The columns' sums: a wave holds ST * 32 keys, the block streams the queries that see any of them, head by head.
-// grid: x blocks of keys (of the longest segment), y kv heads * splits of the (head, stage of queries) pairs, z segments.
+// grid: x kv heads times blocks of keys (of the longest segment), y splits of the (head, stage of queries) pairs, z segments.
 // part [splits, kv heads, places]; a segment's places begin at list.off.
 template <typename T, int DHP, int ST>
 __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
                                                                        const float* __restrict__ lse, float* __restrict__ part, int splits, long places) {
-    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, STAGE_BYTES = PT_STAGE * PPR * 16, KEYS = 32 * ST;
+    constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16, KEYS = 32 * ST;
+    constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int which = blockIdx.z, seg = list.seg[which], kvh = blockIdx.y / splits, split = blockIdx.y % splits;
+    const int which = blockIdx.z, seg = list.seg[which], kvh = blockIdx.x % a.nkv, split = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
     const int nq = list.q[which], ctx = list.ctx[which], base = ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE, tok0 = list.start[which];
-    const int b0 = blockIdx.x * KEYS * PT_WAVES, k0 = b0 + w * KEYS;
+    const int b0 = blockIdx.x / a.nkv * KEYS * PT_WAVES, k0 = b0 + w * KEYS;
     if (b0 >= ctx) return;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
     if (pieces < PPR) {
-        for (int i = tid; i < 2 * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
+        for (int i = tid; i < PT_BUFS * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
         __syncthreads();
     }
     u32x4_t kf[ST][CH];
@@ -447,74 +541,95 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
 #pragma unroll
         for (int j = 0; j < CH; ++j) kf[x][j] = 2 * j + half < pieces ? *reinterpret_cast<const u32x4_t*>(src + (2 * j + half) * PE) : u32x4_t{0, 0, 0, 0};
     }
-    float sums[ST][16];
+    f32x16_t sums[ST];
 #pragma unroll
     for (int x = 0; x < ST; ++x)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sums[x][r] = 0.f;
     // pairs (head, stage of queries), numbered head by head; this split's share of them
-    const int first = max(b0 - base, 0) / PT_STAGE, n = (nq + PT_STAGE - 1) / PT_STAGE - first;
+    const int first = max(b0 - base, 0) / ROWS, n = (nq + ROWS - 1) / ROWS - first;
     const int u0 = (int)((long)rep * n * split / splits), u1 = (int)((long)rep * n * (split + 1) / splits);
     int lh = u0 / n, ls = first + u0 % n;                // the pair that is loaded next
-    auto load = [&](int buf) {
-        const T* src = q + (size_t)(kvh * rep + lh) * a.dh;
-        const int i0 = ls * PT_STAGE;
-        stage_rows<PPR>(lds + buf * STAGE_BYTES, pieces, w, lane, [&](int r) {
-            return (const char*)(src + (size_t)(tok0 + min(i0 + r, nq - 1)) * a.q_row_stride);
-        });
-    };
-    float lnext[PT_STAGE / 32];
-    auto load_lse = [&]() {
+    const uint32_t q_pieces = a.q_row_stride / PE;
+    float lq[PT_BUFS][TPS];                              // the queries' lse of the stages on their way, and where these begin
+    int from[PT_BUFS];
+    auto load = [&](auto which_buf) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which_buf)::value;
+        const int i0 = ls * ROWS;
+        from[buf] = i0;
 #pragma unroll
-        for (int y = 0; y < PT_STAGE / 32; ++y) {
-            const int i = ls * PT_STAGE + 32 * y + c;
-            lnext[y] = i < nq ? lse[(size_t)(tok0 + i) * a.nh + kvh * rep + lh] : INFINITY;
+        for (int y = 0; y < TPS; ++y) {
+            const int i = i0 + 32 * y + c;
+            lq[buf][y] = i < nq ? lse[(tok0 + i) * a.nh + kvh * rep + lh] : INFINITY;
         }
+        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, q, pieces, w, lane, [&](int r) {
+            return (uint32_t)(tok0 + min(i0 + r, nq - 1)) * q_pieces + (kvh * rep + lh) * pieces;
+        });
+        if (++ls == first + n) { ls = first; ++lh; }
     };
-    auto advance = [&]() { if (++ls == first + n) { ls = first; ++lh; } };
-    int cs = ls;
-    if (u0 < u1) { load_lse(); load(0); advance(); }
-    for (int u = u0; u < u1; ++u) {
-        const int buf = (u - u0) & 1, i0 = cs * PT_STAGE;
-        float lq[PT_STAGE / 32];
+    int at[CH];
+    staged_at<PPR>(c, half, at);
+    u32x4_t ring[PT_RING];
+    auto share = [&](const f32x16_t (&acc)[ST], float lq, int j) __attribute__((always_inline)) {       // a tile's sums, in CH shares
 #pragma unroll
-        for (int y = 0; y < PT_STAGE / 32; ++y) lq[y] = lnext[y];
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        cs = ls;
-        if (u + 1 < u1) { load_lse(); load(buf ^ 1); advance(); }
-        const char* st = lds + buf * STAGE_BYTES;
+        for (int x = 0; x < ST; ++x)
 #pragma unroll
-        for (int y = 0; y < PT_STAGE / 32; ++y) {
-            const int q0 = i0 + 32 * y;                  // the tile's first query
-            if (q0 >= nq || base + q0 + 31 < k0) continue;
-            f32x16_t acc[ST];
+            for (int r = 0; r < 16; ++r)
+                if ((16 * x + r) * CH / (16 * ST) == j) sums[x][r] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq));
+    };
+    // a tile whose queries do not all see all the wave's keys is added up at once, and leaves nothing for later
+    auto hide = [&](f32x16_t (&acc)[ST], float& lq, int q0) __attribute__((always_inline)) {
+        if (base + q0 >= k0 + KEYS - 1 && q0 < nq) return;
+        const int pos = base + q0 + c;
+        if (q0 < nq && base + q0 + 31 >= k0)
 #pragma unroll
             for (int x = 0; x < ST; ++x)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq));
+                    sums[x][r] += k0 + 32 * x + 4 * half + 8 * (r >> 2) + (r & 3) <= pos ? e : 0.f;
+                }
+        nothing<ST>(acc);
+        lq = 0.f;
+    };
+    auto stay = [&]() __attribute__((always_inline)) {   // (the compiler would move the exponentials behind the branch that follows)
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const u32x4_t qf = staged_piece<PPR>(st, 32 * y + c, 2 * j + half);
-#pragma unroll
-                for (int x = 0; x < ST; ++x) acc[x] = mma32<T>(kf[x][j], qf, acc[x]);
-            }
-            if (base + q0 >= k0 + KEYS - 1) {            // every query sees every key
-#pragma unroll
-                for (int x = 0; x < ST; ++x)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sums[x][r] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq[y]));
-            } else {
-                const int pos = base + q0 + c;
-#pragma unroll
-                for (int x = 0; x < ST; ++x)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -lq[y]));
-                        sums[x][r] += k0 + 32 * x + 4 * half + 8 * (r >> 2) + (r & 3) <= pos ? e : 0.f;
-                    }
-            }
+        for (int x = 0; x < ST; ++x) asm volatile("" : "+v"(sums[x]));
+    };
+    f32x16_t acc[2][ST];
+    float lacc[2] = {0.f, 0.f};
+    nothing<ST>(acc[0]);
+    nothing<ST>(acc[1]);
+    if (u0 < u1) {
+        load(std::integral_constant<int, 0>{});
+        if (u0 + 1 < u1) {
+            load(std::integral_constant<int, 1>{});
+            arrived<LOADS>();
+        } else {
+            arrived<0>();
         }
+#pragma unroll
+        for (int j = 0; j < PT_RING; ++j) ring[j] = staged_piece(lds, at[j]);
+    }
+    const int steps = (u1 - u0) * TPS;
+    in_steps(steps, [&](auto index, int t) __attribute__((always_inline)) {
+        constexpr int I = decltype(index)::value, buf = I / TPS % PT_BUFS, y = I % TPS, nbuf = (I + 1) / TPS % PT_BUFS, ny = (I + 1) % TPS, now = I & 1;
+        const int u = u0 + t / TPS;
+        if (y == TPS - 1 && u + 1 < u1) {                // the next stage is there, and nobody reads the one before this any more
+            arrived<0>();
+            if (u + 2 < u1) load(std::integral_constant<int, (buf + 2) % PT_BUFS>{});
+        }
+        multiply_rows<CH, ST>(lds + buf * STAGE_BYTES + 32 * y * PPR * 16, lds + nbuf * STAGE_BYTES + 32 * ny * PPR * 16, at, ring, kf, acc[now],
+                              [](const u32x4_t staged, const u32x4_t held, f32x16_t v) { return mma32<T>(held, staged, v); },
+                              [&](int j) __attribute__((always_inline)) { share(acc[now ^ 1], lacc[now ^ 1], j); });
+        stay();
+        lacc[now] = lq[buf][y];
+        hide(acc[now], lacc[now], from[buf] + 32 * y);
+    });
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {                       // the last tile's
+        if (steps & 1) share(acc[0], lacc[0], j);
+        else share(acc[1], lacc[1], j);
     }
     float* out = part + ((size_t)split * a.nkv + kvh) * places + list.off[blockIdx.z];
 #pragma unroll
@@ -537,7 +652,12 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list
     if (row < 0) return;
     const float* src = part + (size_t)kvh * places + list.off[blockIdx.z] + t;
     float sum = 0.f;
-    for (int s = 0; s < splits; ++s) sum += src[(size_t)s * a.nkv * places];
+    for (int s = 0; s < splits; s += 4) {                // (four on their way at a time)
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = s + i < splits ? src[(size_t)(s + i) * a.nkv * places] : 0.f;
+        sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
     mass[row] = a.fresh && t >= ctx - list.q[blockIdx.z] ? sum : mass[row] + sum;
 }
 
@@ -547,7 +667,7 @@ struct MassPlan {
     int single_ctx = 0, multi_ctx = 0, multi_q = 0;
     long stride = 0;                     // keys of a head's scores
     int parts = 0;
-    int row_splits = 1, key_splits = 1, st = 1;
+    int row_splits = 1, key_splits = 1, row_st = 1;
     long places = 0;                     // of the longer segments' sums, all together
     long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
     bool tiled = false, valid = false;
@@ -555,9 +675,10 @@ struct MassPlan {
 
 struct Batch { const int *q_start, *q_len, *ctx_len; };      // in host memory
 
-static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, const void* k, float scale) {
+// (the tiles' loads count pieces of 16 bytes in 32 bits)
+static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, const void* k, float scale, long tokens, long nh, long rows) {
     const int es = dtype == LI_BF16 ? 2 : 4;
-    return dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
+    return tokens * (q_row_stride * (long)es / 16) < 1L << 32 && rows * (dh * es / 16) < 1L << 32 && tokens * nh < 1L << 31 && dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
 }
 
 static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, bool f32, bool tiled) {
@@ -592,12 +713,18 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
         p.floats = p.stats + 2L * p.single * nh * p.parts;
     }
     if (p.multi) {
-        p.st = f32 ? 1 : 2;
-        const long row_blocks = ((long)(p.multi_q + 32 * p.st - 1) / (32 * p.st) * rep + PT_WAVES - 1) / PT_WAVES * nkv * p.multi;
-        const int stages = (p.multi_ctx + PT_STAGE - 1) / PT_STAGE;
-        while (p.row_splits < 16 && row_blocks * p.row_splits < 512 && stages / (2 * p.row_splits) >= 4) p.row_splits *= 2;
-        const long key_blocks = pairs * nkv, units = (long)rep * ((p.multi_q + PT_STAGE - 1) / PT_STAGE);
-        while (p.key_splits < 16 && key_blocks * p.key_splits < 1024 && units / (2 * p.key_splits) >= 2) p.key_splits *= 2;
+        // Blocks enough for some rounds over the compute units (two a unit at a time), each long enough to be worth its start: 1,999 queries of 40
+        // heads behind 16,000 keys, rows / columns at 512, 1,024 and 1,536 blocks 534, 478, 484 / 483, 440, 428 us.
+        // Rows: a wave holds two tiles of queries where that leaves two blocks a unit, else one (2,048 queries of 28 heads 37 us, with two 44;
+        // 1,999 behind 16,000 520 and 478).
+        const int stages = (p.multi_ctx + 63) / 64;
+        for (p.row_st = f32 ? 1 : 2;; p.row_st = 1) {
+            const long blocks = ((long)(p.multi_q + 32 * p.row_st - 1) / (32 * p.row_st) * rep + PT_WAVES - 1) / PT_WAVES * nkv * p.multi;
+            for (p.row_splits = 1; p.row_splits < 16 && blocks * p.row_splits < 1024 && stages / (2 * p.row_splits) >= 8;) p.row_splits *= 2;
+            if (p.row_st == 1 || blocks * p.row_splits >= 512) break;
+        }
+        const long key_blocks = pairs * nkv, units = (long)rep * ((p.multi_q + 63) / 64);
+        while (p.key_splits < 16 && key_blocks * p.key_splits < 1536 && units / (2 * p.key_splits) >= 2) p.key_splits *= 2;
         p.rows = p.floats;
         p.lse = p.rows + 2L * p.row_splits * tokens * nh;
         p.sums = p.lse + (long)tokens * nh;
@@ -607,11 +734,11 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
 }
 
 // Floats of workspace for a batch (its segments in host memory); -1: not a batch.  padded_ctx > 0: a batch that is recorded and replayed
-// for any contexts up to that.  q, k: the addresses, whose alignment decides on the kernel.
+// for any contexts up to that.  q, k: the addresses, whose alignment decides on the kernel; rows: pages * nkv * page_size.
 extern "C" long li_attention_mass_work_floats(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, int dtype,
-                                              int q_row_stride, const void* q, const void* k, float scale) {
+                                              int q_row_stride, const void* q, const void* k, float scale, long rows) {
     if (nseg <= 0 || tokens <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || !q_len || !ctx_len) return -1;
-    const MassPlan p = mass_plan(q_len, ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, k, scale));
+    const MassPlan p = mass_plan(q_len, ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, k, scale, tokens, nh, rows));
     return p.valid ? p.floats : -1;
 }
 
@@ -624,7 +751,7 @@ template <typename T, int DHP>
 static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg,
                              int tokens, float* work, hipStream_t stream) {
     constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1, KEYS = 32 * ST * PT_WAVES;
-    constexpr int LDS_BYTES = 2 * PT_STAGE * DHP * (int)sizeof(T);
+    constexpr int LDS_BYTES = PT_BUFS * 32 * stage_tiles(DHP * (int)sizeof(T)) * DHP * (int)sizeof(T);
     if (p.single) {
         for (int at = 0, i = 0; at < p.single;) {
             SegList list;
@@ -647,10 +774,10 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
         }
     }
     if (p.multi) {
-        const auto rows = mass_rows_tile_kernel<T, DHP, ST>;
+        const auto rows = p.row_st == ST ? mass_rows_tile_kernel<T, DHP, ST> : mass_rows_tile_kernel<T, DHP, 1>;
         const auto keys = mass_keys_tile_kernel<T, DHP, ST>;
         if (!allow_lds(rows, LDS_BYTES) || !allow_lds(keys, LDS_BYTES)) return LI_ERR_LAUNCH;
-        const int rep = a.nh / a.nkv, tiles = (p.multi_q + 32 * ST - 1) / (32 * ST);
+        const int rep = a.nh / a.nkv, tiles = (p.multi_q + 32 * p.row_st - 1) / (32 * p.row_st);
         float2* stats = (float2*)(work + p.rows);
         float *lse = work + p.lse, *sums = work + p.sums;
         const long rows_n = (long)tokens * a.nh;
@@ -667,15 +794,15 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                 list.n = n;
                 at += n;
                 if (pass == 0) {
-                    rows<<<dim3((tiles * rep + PT_WAVES - 1) / PT_WAVES, a.nkv, n * p.row_splits), 64 * PT_WAVES, LDS_BYTES, stream>>>(
-                        q, k, a, list, stats, p.row_splits, tokens);
+                    rows<<<dim3((tiles * rep + PT_WAVES - 1) / PT_WAVES * a.nkv, 1, n * p.row_splits), 64 * PT_WAVES, LDS_BYTES, stream>>>(
+                        q, k, a, list, stats, lse, p.row_splits, tokens);
                 } else {
-                    keys<<<dim3((p.multi_ctx + KEYS - 1) / KEYS, a.nkv * p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
+                    keys<<<dim3((p.multi_ctx + KEYS - 1) / KEYS * a.nkv, p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
                         q, k, a, list, lse, sums, p.key_splits, p.places);
                     mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, p.key_splits, p.places, mass);
                 }
             }
-            if (pass == 0) mass_lse_kernel<<<(unsigned)((rows_n + 255) / 256), 256, 0, stream>>>(stats, p.row_splits, rows_n, lse);
+            if (pass == 0 && p.row_splits > 1) mass_lse_kernel<<<(unsigned)((rows_n + 255) / 256), 256, 0, stream>>>(stats, p.row_splits, rows_n, lse);
         }
     }
     return li_launch_status();
@@ -700,7 +827,8 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
                                  int padded_ctx, int nh, int nkv, int dh, int page_size, int num_pages, float scale, int fresh, float* work,
                                  hipStream_t stream) {
     if (nseg <= 0 || nseg > 65535 || tokens <= 0 || nh <= 0 || nh > 65535 || nkv <= 0 || nkv > 4095 || nh % nkv || dh <= 0 || dh > EV_MAX_DH || page_size <= 0 ||
-        max_blocks <= 0 || (long)max_blocks * page_size >= 1L << 31 || num_pages <= 0 || !h_q_start || !h_q_len || !h_ctx_len || !work)
+        max_blocks <= 0 || (long)max_blocks * page_size >= 1L << 31 || num_pages <= 0 ||
+        (long)num_pages * nkv * page_size >= 1L << 31 || !h_q_start || !h_q_len || !h_ctx_len || !work)
         return LI_ERR_SIZE;
     const long room = (long)max_blocks * page_size;
     for (int i = 0; i < nseg; ++i)
@@ -708,7 +836,7 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
     if (dtype != LI_F32 && dtype != LI_BF16) return LI_ERR_DTYPE;
     const MassArgs a = {block_table, q_start, q_len, ctx_len, max_blocks, nh, nkv, dh, page_size, num_pages, q_row_stride,
                         (uint32_t)(page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size)), scale * 1.44269504088896341f, fresh};
-    const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale));
+    const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale, tokens, nh, (long)num_pages * nkv * page_size));
     if (!p.valid) return LI_ERR_SIZE;
     const Batch b = {h_q_start, h_q_len, h_ctx_len};
     if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, nseg, tokens, work, stream);

@@ -2010,7 +2010,8 @@ def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta,
     # (a recorded step is replayed for longer contexts of the same tables)
     padded = meta.max_blocks * page_size if meta.padded else 0
     dt, hq, hc = _DT[qkv.dtype], hq.ctypes.data, hc.ctypes.data
-    need = _mass_work_floats()(hq, hc, n, t, padded, nh, nkv, dh, dt, qkv.stride(0), qkv.data_ptr(), k.data_ptr(), float(scale))
+    need = _mass_work_floats()(hq, hc, n, t, padded, nh, nkv, dh, dt, qkv.stride(0), qkv.data_ptr(), k.data_ptr(), float(scale),
+                              k.shape[0] * nkv * page_size)
     _chk(need >= 0, "attention_mass: the segments' lengths are not those of a batch")
     work = ws.buffer("evict.mass", (need,), torch.float32) if ws is not None else _scratch.floats(need, qkv.device)
     _run("evict", "li_attention_mass", qkv.data_ptr(), qkv.stride(0), k.data_ptr(), mass.data_ptr(), dt, bt.data_ptr(), meta.max_blocks,
@@ -2019,7 +2020,7 @@ def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta,
 
 
 def _mass_work_floats():
-    return _lib_fn("evict", "li_attention_mass_work_floats", [P, P] + [I] * 8 + [P, P, F], c_long)
+    return _lib_fn("evict", "li_attention_mass_work_floats", [P, P] + [I] * 8 + [P, P, F, L], c_long)
 
 
 def _check_requests(what: str, block_table, n: int, page_size: int) -> None:
