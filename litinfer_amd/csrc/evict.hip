@@ -156,23 +156,17 @@ __device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x
 #define SG_KEYS 64                // keys of a wave
 #define SG_WAVES 4
 
-// Scores of 64 keys a wave against the heads of a kv head, 16 at a time, and the wave's maximum and sum for every head.
-// scores [request, nh, stride], stats [request, nh, parts] of (m, l).
+// Scores of the 64 keys from k0 on against the heads of a kv head, 16 at a time, by a wave, and the maximum and sum for every head:
+// scores [head of the kv head, stride] from key k0 on, stats [head, parts].
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                           float* __restrict__ scores, long stride, float2* __restrict__ stats, int parts) {
+__device__ __forceinline__ void single_scores(const T* __restrict__ qrow, const T* __restrict__ k, const MassArgs& a, const int* table, int kvh, int k0, int ctx,
+                                              int lane, float* scores, long stride, float2* stats, int parts) {
     constexpr int PE = 16 / sizeof(T);                   // elements of a piece
     constexpr int NT = CH * 4 <= 16 ? 4 : CH * 2 <= 16 ? 2 : 1;      // tiles of 16 keys whose pieces are asked for at once
-    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int part = blockIdx.x * SG_WAVES + (threadIdx.x >> 6), k0 = part * SG_KEYS;
-    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS);
-    if (k0 >= ctx) return;
-    const int* table = a.block_table + (size_t)seg * a.max_blocks;
-    const int rep = a.nh / a.nkv, dh = a.dh;
+    const int c = lane & 15, g = lane >> 4, rep = a.nh / a.nkv, dh = a.dh;
     long row[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) row[i] = k0 + 16 * i + c < ctx ? place_row(a, table, kvh, k0 + 16 * i + c) : -1;
-    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * dh;
     const u32x4_t zero = {0, 0, 0, 0};
     for (int h0 = 0; h0 < rep; h0 += 16) {
         u32x4_t qf[CH];
@@ -220,13 +214,25 @@ __global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const
             for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(s[i][r] - base);
         l = lane_xor_add(lane_xor_add(l, 16), 32);
         if (h0 + c < rep) {
-            const size_t head = (size_t)req * a.nh + (size_t)kvh * rep + h0 + c;
-            float* out = scores + head * stride + k0 + 4 * g;
+            float* out = scores + (size_t)(h0 + c) * stride + k0 + 4 * g;
 #pragma unroll
             for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4_t*>(out + 16 * i) = s[i];      // (stride: whole runs of 64)
-            if (g == 0) stats[head * parts + part] = make_float2(m, l);
+            if (g == 0) stats[(size_t)(h0 + c) * parts + k0 / SG_KEYS] = make_float2(m, l);
         }
     }
+}
+
+// grid: x runs of 64 keys / 4, y kv heads, z requests; scores [request, nh, stride], stats [request, nh, parts].
+template <typename T, int CH>
+__global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
+                                                                           float* __restrict__ scores, long stride, float2* __restrict__ stats, int parts) {
+    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, rep = a.nh / a.nkv;
+    const int k0 = (blockIdx.x * SG_WAVES + (threadIdx.x >> 6)) * SG_KEYS;
+    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS);
+    if (k0 >= ctx) return;
+    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    const size_t head0 = (size_t)req * a.nh + (size_t)kvh * rep;
+    single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)seg * a.max_blocks, kvh, k0, ctx, lane, scores + head0 * stride, stride, stats + head0 * parts, parts);
 }
 
 // lse of a head from the statistics of its `n` parts, by a wave.
@@ -241,6 +247,40 @@ __device__ __forceinline__ float join_stats(const float2* st, int n, int lane) {
     const float mx = wave_max(m);
     l = wave_sum(m == -INFINITY ? l : l * exp2f(m - mx));
     return l == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(l);
+}
+
+// Short contexts: a block takes all of a (request, kv head)'s keys, its scores stay in LDS.  grid: x kv heads, y requests.
+// LDS: scores [rep, stride], stats [rep, stride / 64], lse [rep].
+constexpr int block_waves(int ch) { return ch >= 8 ? 8 : 16; }          // (as many as have the registers for a run of keys)
+template <typename T, int CH>
+__global__ __launch_bounds__(64 * block_waves(CH)) void mass_single_block_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list, int stride,
+                                                                          float* __restrict__ mass) {
+    constexpr int WAVES = block_waves(CH);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int req = blockIdx.y, seg = list.n ? list.seg[req] : req, kvh = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, rep = a.nh / a.nkv;
+    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], stride), parts = stride / SG_KEYS;
+    float* scores = reinterpret_cast<float*>(lds);
+    float2* stats = reinterpret_cast<float2*>(scores + (size_t)rep * stride);
+    float* lse = reinterpret_cast<float*>(stats + rep * parts);
+    const int* table = a.block_table + (size_t)seg * a.max_blocks;
+    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    for (int k0 = w * SG_KEYS; k0 < ctx; k0 += WAVES * SG_KEYS)
+        single_scores<T, CH>(qrow, k, a, table, kvh, k0, ctx, lane, scores, stride, stats, parts);
+    __syncthreads();
+    const int n = (ctx + SG_KEYS - 1) / SG_KEYS;
+    for (int h = w; h < rep; h += WAVES) {
+        const float v = join_stats(stats + h * parts, n, lane);
+        if (lane == 0) lse[h] = v;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < ctx; t += 64 * WAVES) {
+        const long row = place_row(a, table, kvh, t);
+        if (row < 0) continue;
+        const float before = a.fresh && t == ctx - 1 ? 0.f : mass[row];
+        float sum = 0.f;
+        for (int h = 0; h < rep; ++h) sum += __builtin_amdgcn_exp2f(scores[h * stride + t] - lse[h]);
+        mass[row] = before + sum;
+    }
 }
 
 #define SG_LSE 64                 // heads of a kv head whose lse a block holds at a time
@@ -666,7 +706,8 @@ struct MassPlan {
     int single = 0, multi = 0;           // segments of one token, of more
     int single_ctx = 0, multi_ctx = 0, multi_q = 0;
     long stride = 0;                     // keys of a head's scores
-    int parts = 0;
+    int parts = 0, block_lds = 0;
+    bool one_block = false;              // short contexts of single tokens: one kernel
     int row_splits = 1, key_splits = 1, row_st = 1;
     long places = 0;                     // of the longer segments' sums, all together
     long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
@@ -708,9 +749,15 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
     if (p.single) {
         p.parts = (p.single_ctx + SG_KEYS - 1) / SG_KEYS;
         p.stride = (long)p.parts * SG_KEYS;
+        const long lds = 4 * (rep * p.stride + 2L * rep * p.parts + rep);
+        // One kernel where a block has few keys, or where the blocks fill the compute units, us: bfloat16, 28 heads on 4 of 128, one request of 300 keys 9.0
+        // (two kernels) and 6.8, 64 requests 13.3 and 7.1, of 1,000 20.0 and 14.8, of 2,000 32.5 and 25.6; 8 requests of 1,000 9.4 and 12.8, 64
+        // of 2,000 on 2 kv heads 20.3 and 23.5.
+        p.one_block = lds <= 150 * 1024 && (p.single_ctx <= 512 || ((long)p.single * nkv >= 192 && p.single_ctx <= 2048));
+        p.block_lds = (int)lds;
         p.scores = 0;
-        p.stats = (long)p.single * nh * p.stride;
-        p.floats = p.stats + 2L * p.single * nh * p.parts;
+        p.stats = p.one_block ? 0 : (long)p.single * nh * p.stride;
+        p.floats = p.one_block ? 0 : p.stats + 2L * p.single * nh * p.parts;
     }
     if (p.multi) {
         // Blocks enough for some rounds over the compute units (two a unit at a time), each long enough to be worth its start: 1,999 queries of 40
@@ -739,7 +786,7 @@ extern "C" long li_attention_mass_work_floats(const int* q_len, const int* ctx_l
                                               int q_row_stride, const void* q, const void* k, float scale, long rows) {
     if (nseg <= 0 || tokens <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || !q_len || !ctx_len) return -1;
     const MassPlan p = mass_plan(q_len, ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, k, scale, tokens, nh, rows));
-    return p.valid ? p.floats : -1;
+    return p.valid ? (p.floats > 0 ? p.floats : 1) : -1;
 }
 
 template <typename K>
@@ -764,6 +811,13 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                         list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = 1; list.ctx[n] = b.ctx_len[i]; list.off[n++] = 0;
                     }
                 list.n = n;
+            }
+            if (p.one_block) {
+                const auto block = mass_single_block_kernel<T, CH16>;
+                if (!allow_lds(block, p.block_lds)) return LI_ERR_LAUNCH;
+                block<<<dim3(a.nkv, n), 64 * block_waves(CH16), p.block_lds, stream>>>(q, k, a, list, (int)p.stride, mass);
+                at += n;
+                continue;
             }
             float* scores = work + p.scores + (size_t)at * a.nh * p.stride;
             float2* stats = (float2*)(work + p.stats) + (size_t)at * a.nh * p.parts;
@@ -820,12 +874,13 @@ static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, c
 }
 
 // q_start, q_len, ctx_len: the batch's segments on the device; those with h_ the same in host memory.  padded_ctx > 0: the contexts may be others
-// when a recording is replayed, up to that; then every segment brings one token.  work: li_attention_mass_work_floats of the same batch.
+// when a recording is replayed, up to that; then every segment brings one token.  work: li_attention_mass_work_floats of the same batch
+// (no fewer than are found to be wanted: a batch that was changed since is refused).
 extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc, float* mass, int dtype, const int* block_table, int max_blocks,
                                  const int* q_start, const int* q_len, const int* ctx_len, const int* h_q_start, const int* h_q_len,
                                  const int* h_ctx_len, int nseg, int tokens,
                                  int padded_ctx, int nh, int nkv, int dh, int page_size, int num_pages, float scale, int fresh, float* work,
-                                 hipStream_t stream) {
+                                 long work_floats, hipStream_t stream) {
     if (nseg <= 0 || nseg > 65535 || tokens <= 0 || nh <= 0 || nh > 65535 || nkv <= 0 || nkv > 4095 || nh % nkv || dh <= 0 || dh > EV_MAX_DH || page_size <= 0 ||
         max_blocks <= 0 || (long)max_blocks * page_size >= 1L << 31 || num_pages <= 0 ||
         (long)num_pages * nkv * page_size >= 1L << 31 || !h_q_start || !h_q_len || !h_ctx_len || !work)
@@ -837,7 +892,7 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
     const MassArgs a = {block_table, q_start, q_len, ctx_len, max_blocks, nh, nkv, dh, page_size, num_pages, q_row_stride,
                         (uint32_t)(page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size)), scale * 1.44269504088896341f, fresh};
     const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale, tokens, nh, (long)num_pages * nkv * page_size));
-    if (!p.valid) return LI_ERR_SIZE;
+    if (!p.valid || p.floats > work_floats) return LI_ERR_SIZE;
     const Batch b = {h_q_start, h_q_len, h_ctx_len};
     if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, nseg, tokens, work, stream);
     return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, nseg, tokens, work, stream);
