@@ -37,6 +37,7 @@ struct SegList {
     int off[EV_LIST];            // where the segment's places begin among all
 };
 
+static uint32_t inverse_of(int page_size) { return page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size); }
 // place / page_size and the rest: the product with the rounded-down inverse is at most one too small
 __device__ __forceinline__ int page_of(const MassArgs& a, int t, int& rest) {
     int p = (int)__umulhi((uint32_t)t, a.page_inv);
@@ -890,7 +891,7 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
         if (h_ctx_len[i] > room || h_q_start[i] < 0 || (long)h_q_start[i] + h_q_len[i] > tokens || (padded_ctx > 0 && (h_q_len[i] != 1 || padded_ctx > room))) return LI_ERR_SIZE;
     if (dtype != LI_F32 && dtype != LI_BF16) return LI_ERR_DTYPE;
     const MassArgs a = {block_table, q_start, q_len, ctx_len, max_blocks, nh, nkv, dh, page_size, num_pages, q_row_stride,
-                        (uint32_t)(page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size)), scale * 1.44269504088896341f, fresh};
+                        inverse_of(page_size), scale * 1.44269504088896341f, fresh};
     const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale, tokens, nh, (long)num_pages * nkv * page_size));
     if (!p.valid || p.floats > work_floats) return LI_ERR_SIZE;
     const Batch b = {h_q_start, h_q_len, h_ctx_len};
@@ -906,36 +907,203 @@ __device__ __forceinline__ uint32_t mass_order(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-#define SEL_NT 256
+struct SelectArgs {
+    const float* mass;
+    const int *block_table, *lens, *keeps;
+    int max_blocks, first, recent, K, nkv, page_size, num_pages;
+    uint32_t page_inv;
+    int* out;
+};
 
-// A block a (entry, request, kv head).  The m-th largest sum of the places between the first and the last ones is found digit by
-// digit, eight bits a pass, by counting; then one pass in order writes the places.
-__global__ __launch_bounds__(SEL_NT) void evict_select_kernel(const float* __restrict__ mass, const int* __restrict__ block_table, int max_blocks,
-                                                              const int* __restrict__ lens, const int* __restrict__ keeps, int first_n, int recent_n,
-                                                              int* __restrict__ out, int K, int nkv, int page_size, int num_pages) {
+// Places lo .. hi - 1 of a request compete for `want` of its places; the others of its `len` stay anyway.
+struct Contest { int len, lo, hi, want; };
+__device__ __forceinline__ Contest contest_of(const SelectArgs& a, int req) {
+    const int len = (int)min((long)max(a.lens[req], 0), (long)a.max_blocks * a.page_size);
+    const int keep = min(min(max(a.keeps[req], 0), len), a.K), recent = min(a.recent, keep), first = min(a.first, keep - recent);
+    return {len, first, len - recent, keep - recent - first};
+}
+// A place's sum in the order of the floats; 0, as little as there is, where no page holds it.
+__device__ __forceinline__ int page_of(const SelectArgs& a, int t) {
+    const int p = (int)__umulhi((uint32_t)t, a.page_inv);
+    return p + (t - p * a.page_size >= a.page_size ? 1 : 0);
+}
+__device__ __forceinline__ uint32_t place_key(const SelectArgs& a, const float* pool, const int* table, int kvh, int t) {
+    const int p = page_of(a, t), page = table[p];
+    return page < 0 || page >= a.num_pages ? 0u : mass_order(pool[((size_t)page * a.nkv + kvh) * a.page_size + t - p * a.page_size]);
+}
+
+// The sum of the threads' v before this one, and of all of them.  NT threads; smem has a place a wave.
+template <int NT>
+__device__ __forceinline__ int block_before(int v, int* smem, int& all) {
+    constexpr int W = NT / 64;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int up = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(up, o, 64);
+        if (lane >= o) up += x;
+    }
+    __syncthreads();
+    if (lane == 63) smem[w] = up;
+    __syncthreads();
+    int before = up - v;
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const int x = smem[i];
+        if (i < w) before += x;
+        all += x;
+    }
+    return before;
+}
+
+// A block a (entry, request, kv head), a thread VPT places side by side, whose sums it keeps.  The least sum that is taken is found digit by
+// digit: 256 equal parts of the range between the contest's least and its largest are counted in LDS, then those of the part in which the least
+// taken sum lies, and so on, until all of a part is taken or it is a single value, of whose places the lowest are taken.  (Equal parts of
+// the floats' order, not their leading bits: sums lie within a few octaves, and would meet in a few counters.)
+template <int NT, int VPT>
+__global__ __launch_bounds__(NT) void evict_select_kernel(SelectArgs a) {
+    constexpr int W = NT / 64;
+    __shared__ int counts[256], waves[W], part[3];
+    __shared__ uint32_t ends[2][W];
+    const int kvh = blockIdx.x, req = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int* table = a.block_table + (size_t)req * a.max_blocks;
+    const float* pool = a.mass + (size_t)entry * a.num_pages * a.nkv * a.page_size;
+    int* dst = a.out + (((size_t)entry * gridDim.y + req) * a.nkv + kvh) * a.K;
+    const Contest c = contest_of(a, req);
+    const bool choose = c.want > 0 && c.want < c.hi - c.lo;
+    const int t0 = tid * VPT;
+    uint32_t taken = 0;                                   // bit j: place t0 + j stays
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int t = t0 + j;
+        if (t < c.len && (t < c.lo || t >= c.hi || (!choose && c.want > 0))) taken |= 1u << j;
+    }
+    if (choose) {
+        uint32_t key[VPT];                                // 1 + the order of the sums that compete, 0 for the other places
+        float sum[VPT];
+        const int last = c.len - 1;
+        if (a.page_size % 4 == 0) {                       // four places of a page at a time
+            int at[VPT / 4];
+#pragma unroll
+            for (int j = 0; j < VPT / 4; ++j) at[j] = table[page_of(a, min(t0 + 4 * j, last))];
+#pragma unroll
+            for (int j = 0; j < VPT / 4; ++j) {
+                const int t = min(t0 + 4 * j, last) & ~3;
+                const bool there = at[j] >= 0 && at[j] < a.num_pages;
+                const f32x4_t v = *reinterpret_cast<const f32x4_t*>(pool + ((size_t)(there ? at[j] : 0) * a.nkv + kvh) * a.page_size + t - page_of(a, t) * a.page_size);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[4 * j + i] = there ? v[i] : NAN;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int t = min(t0 + j, last), p = page_of(a, t), page = table[p];
+                const bool there = page >= 0 && page < a.num_pages;
+                const float v = pool[((size_t)(there ? page : 0) * a.nkv + kvh) * a.page_size + t - p * a.page_size];
+                sum[j] = there ? v : NAN;
+            }
+        }
+        uint32_t least = ~0u, most = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int t = t0 + j;
+            const bool competes = t >= c.lo && t < c.hi;
+            key[j] = competes ? mass_order(sum[j]) + 1 : 0u;         // (the order's largest, a NaN of the other sign, does not occur)
+            least = min(least, competes ? key[j] : ~0u);
+            most = max(most, key[j]);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            least = min(least, (uint32_t)lane_xor((int)least, o));
+            most = max(most, (uint32_t)lane_xor((int)most, o));
+        }
+        if (lane == 0) { ends[0][w] = least; ends[1][w] = most; }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < W; ++i) { least = min(least, ends[0][i]); most = max(most, ends[1][i]); }
+        uint32_t from = least, span = most - least;       // keys from .. from + span are looked at: all before are not taken, all behind are
+        int left = c.want, held = 0;                      // how many of these are taken; how many they are
+        for (;;) {
+            const int shift = max(24 - __clz(span | 1), 0);
+            for (int i = tid; i < 256; i += NT) counts[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const uint32_t d = key[j] - from;         // (a key of 0 lies far behind)
+                if (d <= span) atomicAdd(&counts[d >> shift], 1);
+            }
+            __syncthreads();
+            if (w == 0) {                                 // from the last part down: the first at which `left` are reached
+                const int c0 = counts[255 - 4 * lane], c1 = counts[254 - 4 * lane], c2 = counts[253 - 4 * lane], c3 = counts[252 - 4 * lane];
+                int up = c0 + c1 + c2 + c3;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int x = __shfl_up(up, o, 64);
+                    if (lane >= o) up += x;
+                }
+                int above = up - (c0 + c1 + c2 + c3);     // in the parts before the lane's own
+                if (above < left && left <= up) {
+                    int p = 255 - 4 * lane, n = c0;
+                    if (above + n < left) { above += n; --p; n = c1; }
+                    if (above + n < left) { above += n; --p; n = c2; }
+                    if (above + n < left) { above += n; --p; n = c3; }
+                    part[0] = p; part[1] = above; part[2] = n;
+                }
+            }
+            __syncthreads();
+            left -= part[1];
+            held = part[2];
+            from += (uint32_t)part[0] << shift;
+            span = min((1u << shift) - 1, most - from);   // (no further than the largest: a key of 0 would be among the next)
+            if (left == held || shift == 0) break;
+        }
+        // all above the part, and of the part all, or, where it is one value, the lowest `left` places
+        int rank = 0, all;
+        if (left != held) {
+            int mine = 0;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) mine += key[j] == from ? 1 : 0;
+            rank = block_before<NT>(mine, waves, all);
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const bool part_of = key[j] >= from && key[j] - from <= span;
+            if (key[j] > from && !part_of) taken |= 1u << j;
+            if (part_of && (left == held || rank++ < left)) taken |= 1u << j;
+        }
+    }
+    int all;
+    int rank = block_before<NT>(__popc(taken), waves, all);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+        if (taken >> j & 1) {
+            if (rank < a.K) dst[rank] = t0 + j;
+            ++rank;
+        }
+    for (int r = all + tid; r < a.K; r += NT) dst[r] = -1;
+}
+
+#define SEL_NT 1024
+
+// Requests that are longer than a block's registers: the sums are read again for every digit, eight bits of them, the digits counted in LDS.
+__global__ __launch_bounds__(SEL_NT) void evict_select_long_kernel(SelectArgs a) {
     __shared__ int hist[256], wsum[SEL_NT / 64], pick[2];
-    const int kvh = blockIdx.x, req = blockIdx.y, entry = blockIdx.z, nreq = gridDim.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int* table = block_table + (size_t)req * max_blocks;
-    const float* pool = mass + (size_t)entry * num_pages * nkv * page_size;
-    int* dst = out + (((size_t)entry * nreq + req) * nkv + kvh) * K;
-    const long room = (long)max_blocks * page_size;
-    const int len = (int)min((long)max(lens[req], 0), room);
-    const int keep = min(min(max(keeps[req], 0), len), K);
-    const int recent = min(recent_n, keep), first = min(first_n, keep - recent), lo = first, hi = len - recent;
-    const int want = keep - recent - first;              // places chosen by their sums among lo .. hi - 1
-    auto key = [&](int t) {
-        const int page = table[t / page_size];
-        return page < 0 || page >= num_pages ? 0u : mass_order(pool[((size_t)page * nkv + kvh) * page_size + t % page_size]);
-    };
+    const int kvh = blockIdx.x, req = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int* table = a.block_table + (size_t)req * a.max_blocks;
+    const float* pool = a.mass + (size_t)entry * a.num_pages * a.nkv * a.page_size;
+    int* dst = a.out + (((size_t)entry * gridDim.y + req) * a.nkv + kvh) * a.K;
+    const Contest c = contest_of(a, req);
     uint32_t prefix = 0, known = 0;
-    int left = want;                                     // how many are still to be taken among those with the prefix
-    if (want > 0 && want < hi - lo)
+    int left = c.want;                                   // how many are still to be taken among those with the prefix
+    const bool all = c.want >= c.hi - c.lo;
+    if (c.want > 0 && !all)
         for (int shift = 24; shift >= 0; shift -= 8) {
             __syncthreads();
-            hist[tid] = 0;
+            if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int t = lo + tid; t < hi; t += SEL_NT) {
-                const uint32_t u = key(t);
+            for (int t = c.lo + tid; t < c.hi; t += SEL_NT) {
+                const uint32_t u = place_key(a, pool, table, kvh, t);
                 if ((u & known) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
             }
             __syncthreads();
@@ -950,15 +1118,14 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(const float* __res
             known |= 255u << shift;
             left = pick[1];
         }
-    const bool all = want >= hi - lo;
     int at = 0, ties = 0;                                // places written, places equal to the last one taken
-    for (int t0 = 0; t0 < len; t0 += SEL_NT) {
+    for (int t0 = 0; t0 < c.len; t0 += SEL_NT) {
         const int t = t0 + tid;
         bool in = false, tie = false;
-        if (t < len) {
-            if (t < lo || t >= hi || all) in = true;
-            else if (want > 0) {
-                const uint32_t u = key(t);
+        if (t < c.len) {
+            if (t < c.lo || t >= c.hi || all) in = true;
+            else if (c.want > 0) {
+                const uint32_t u = place_key(a, pool, table, kvh, t);
                 in = u > prefix;
                 tie = u == prefix;
             }
@@ -982,18 +1149,25 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(const float* __res
             if (i < w) pos += wsum[i];
             at += wsum[i];
         }
-        if (in && pos < K) dst[pos] = t;
+        if (in && pos < a.K) dst[pos] = t;
     }
-    for (int j = at + tid; j < K; j += SEL_NT) dst[j] = -1;
+    for (int j = at + tid; j < a.K; j += SEL_NT) dst[j] = -1;
 }
 
 // mass [entries, num_pages, nkv, page_size]; lens, keeps [n]; out [entries, n, nkv, K], ascending, -1 behind the last.
 extern "C" int li_evict_select(const float* mass, const int* block_table, int max_blocks, const int* lens, const int* keeps, int n, int first, int recent,
                                int* out, int K, int entries, int nkv, int page_size, int num_pages, hipStream_t stream) {
-    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || first < 0 || recent < 0 || max_blocks <= 0 || page_size <= 0 ||
+    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || first < 0 || recent < 0 || max_blocks <= 0 || num_pages <= 0 || page_size <= 0 ||
         (long)max_blocks * page_size >= 1L << 31)
         return LI_ERR_SIZE;
-    evict_select_kernel<<<dim3(nkv, n, entries), SEL_NT, 0, stream>>>(mass, block_table, max_blocks, lens, keeps, first, recent, out, K, nkv, page_size, num_pages);
+    const SelectArgs a = {mass, block_table, lens, keeps, max_blocks, first, recent, K, nkv, page_size, num_pages, inverse_of(page_size), out};
+    const long room = (long)max_blocks * page_size;      // (as long as any request can be; the tables say no more)
+    const dim3 grid(nkv, n, entries);
+    if (room <= 1024) evict_select_kernel<256, 4><<<grid, 256, 0, stream>>>(a);
+    else if (room <= 4096) evict_select_kernel<256, 16><<<grid, 256, 0, stream>>>(a);
+    else if (room <= 16384) evict_select_kernel<1024, 16><<<grid, 1024, 0, stream>>>(a);
+    else if (room <= 32768) evict_select_kernel<1024, 32><<<grid, 1024, 0, stream>>>(a);
+    else evict_select_long_kernel<<<grid, SEL_NT, 0, stream>>>(a);
     return li_launch_status();
 }
 

@@ -27,6 +27,20 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float float_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+// Logits e .. e + 3 of a row of V, -inf behind its end.
+__device__ __forceinline__ void load_four(const float* src, int e, int V, float (&v)[4]) {
+    if (e + 3 < V) {
+        const f32x4u y = *reinterpret_cast<const f32x4u*>(src + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = y[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = e + j < V ? src[e + j] : -INFINITY;
+    }
+}
+
 template <int U>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprob_rows_kernel(const float* __restrict__ x, long stride, int V, int shares,
                                                                      RowShare* __restrict__ out, float* __restrict__ tops, int groups) {
@@ -38,15 +52,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_rows_kernel(const float
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int e = at + u * LP_GROUP + 4 * lane;
-        if (e + 3 < V) {
-            const f32x4u y = *reinterpret_cast<const f32x4u*>(src + e);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[u][j] = y[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[u][j] = e + j < V ? src[e + j] : -INFINITY;
-        }
+        load_four(src, at + u * LP_GROUP + 4 * lane, V, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -99,72 +105,179 @@ __device__ __forceinline__ uint64_t block_max64(uint64_t v, uint64_t* smem) {
     return b;
 }
 
-// One block a row: joins the waves' shares, then finds the likeliest tokens.
+// How many of the block's threads' values are counted by f, in every thread; `turn` alternates between calls (one barrier each).
+template <typename F>
+__device__ __forceinline__ int block_count(int n, int (*smem)[LP_WAVES], int turn, F f) {
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += 64 * LP_WAVES) c += __popcll(__ballot(f(i)));      // (of the lanes that are still in the loop)
+    if ((threadIdx.x & 63) == 0) smem[turn & 1][threadIdx.x >> 6] = c;       // (the wave's first lane leaves the loop last)
+    __syncthreads();
+    return smem[turn & 1][0] + smem[turn & 1][1] + smem[turn & 1][2] + smem[turn & 1][3];
+}
+
+// One block a row: joins the waves' shares, then finds the likeliest tokens.  A value that at least k and at most LP_LIST groups' maxima
+// reach is found by halving the range between the least and the largest; the logits of these groups that reach it are gathered (at least
+// k, seldom many more) and each one's rank counted.  Where many values are equal or likely tokens lie side by side no such value may exist, or more
+// logits reach it than there is room for: then the k first are taken one after the other.
+#define LP_LIST 64                // groups that are looked through
+#define LP_ROOM 256               // logits that are ranked
 __global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float* __restrict__ x, long stride, int V, int shares,
                                                                      const RowShare* __restrict__ in, const float* __restrict__ tops, int groups,
                                                                      const int* __restrict__ ids, float* __restrict__ logprob,
                                                                      float* __restrict__ entropy, int top, int* __restrict__ top_ids,
                                                                      float* __restrict__ top_logprob) {
     constexpr int NT = 64 * LP_WAVES;
-    __shared__ float red[LP_WAVES];
-    __shared__ uint64_t red64[LP_WAVES];
-    __shared__ int chosen[LP_MAX_TOP];
-    const int row = blockIdx.x, tid = threadIdx.x;
+    __shared__ float red[LP_WAVES], sums[LP_WAVES][3];
+    __shared__ uint64_t red64[LP_WAVES], list[LP_ROOM];
+    __shared__ int chosen[LP_LIST], counts[2][LP_WAVES], found;
+    extern __shared__ uint32_t keys[];                    // the groups' maxima, in their order (and room for the k first groups' logits)
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const float* src = x + (size_t)row * stride;
     in += (size_t)row * shares;
-    float m = -INFINITY;
-    for (int i = tid; i < shares; i += NT) m = fmaxf(m, in[i].m);
+    // (what is read from memory is asked for before the first of it is waited for)
+    const RowShare none = {-INFINITY, 0.f, 0.f, 0.f}, first = tid < shares ? in[tid] : none;
+    const int id = ids[row];
+    const float given = id >= 0 && id < V ? src[id] : NAN;
+    if (top) {
+        tops += (size_t)row * groups;
+        for (int i = tid; i < groups; i += NT) keys[i] = order_of(tops[i]);
+        if (tid == 0) found = 0;
+    }
+    float m = first.m;
+    for (int i = tid + NT; i < shares; i += NT) m = fmaxf(m, in[i].m);
     m = wave_max(m);
-    if ((tid & 63) == 0) red[tid >> 6] = m;
+    if (lane == 0) red[w] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float c = 0.f, r = 0.f, t = 0.f;
     for (int i = tid; i < shares; i += NT) {
-        const RowShare s = in[i];
+        const RowShare s = i == tid ? first : in[i];
         if (s.m == m) { c += s.c; r += s.r; t += s.t; continue; }
         const float d = fmaxf(s.m - m, -1e30f), e = expf(s.m - m);
         r += e * (s.c + s.r);
         t += e * (s.t + (s.c + s.r) * d);
     }
-    c = block_sum<NT>(c, red);
-    r = block_sum<NT>(r, red);
-    t = block_sum<NT>(t, red);
+    c = wave_sum(c);
+    r = wave_sum(r);
+    t = wave_sum(t);
+    if (lane == 0) { sums[w][0] = c; sums[w][1] = r; sums[w][2] = t; }
+    __syncthreads();
+    c = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
+    r = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
+    t = (sums[0][2] + sums[1][2]) + (sums[2][2] + sums[3][2]);
     // (a maximum that is not finite leaves no probabilities)
     const float log_s = fabsf(m) < INFINITY ? logf(c) + log1pf(r / c) : NAN;
     if (tid == 0) {
-        const int id = ids[row];
-        logprob[row] = id >= 0 && id < V ? (src[id] - m) - log_s : NAN;
+        logprob[row] = (given - m) - log_s;
         entropy[row] = log_s - t / (c + r);
     }
     if (!top) return;
-    // the groups with the k first maxima, one after the other
-    tops += (size_t)row * groups;
+    // lo is reached by at least `want` groups, hi by fewer (rows of fewer groups than tokens are wanted: by all of them)
+    const int want = top < groups ? top : groups;
+    uint32_t lo = 0, hi = order_of(m);
+    int n = groups, turn = 0;
+    if (top == 1) {
+        lo = hi;
+        n = 1;
+    } else {
+        // (likely tokens lie a few nats below the first: four tries there, then halves)
+        const int enough = min(LP_LIST, want + max(4, want / 2));
+        for (float d = 2.f; n > enough && d < 64.f && fabsf(m) < 1e30f; d *= 2.5f) {
+            const uint32_t mid = order_of(m - d);
+            if (mid <= lo || mid >= hi) break;
+            const int reach = block_count(groups, counts, turn++, [&](int i) { return keys[i] >= mid; });
+            if (reach >= want) { lo = mid; n = reach; break; }
+            hi = mid;
+        }
+        while (n > enough && hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int reach = block_count(groups, counts, turn++, [&](int i) { return keys[i] >= mid; });
+            if (reach >= want) { lo = mid; n = reach; } else hi = mid;
+        }
+    }
+    bool ranked = n <= LP_LIST;
+    if (ranked) {
+        // the groups in any order, then their logits that reach lo
+        for (int i = tid; i < groups; i += NT)
+            if (keys[i] >= lo) {
+                const int at = atomicAdd(&found, 1);
+                if (at < LP_LIST) chosen[at] = i;
+            }
+        __syncthreads();
+        const int held = found;
+        ranked = held <= LP_LIST;                         // (one maximum may be many groups')
+        __syncthreads();
+        if (tid == 0) found = 0;
+        __syncthreads();
+        if (ranked) {
+            constexpr int AT_ONCE = 4;                    // groups of a wave that are on their way together
+            for (int g0 = w; g0 < held; g0 += AT_ONCE * LP_WAVES) {
+                float v[AT_ONCE][4];
+                int from[AT_ONCE];
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) {
+                    const int g = g0 + i * LP_WAVES;
+                    from[i] = g < held ? chosen[g] * LP_GROUP + 4 * lane : V;
+                    load_four(src, from[i], V, v[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t u = order_of(v[i][j]);
+                        if (from[i] + j < V && u >= lo) {
+                            const int at = atomicAdd(&found, 1);
+                            if (at < LP_ROOM) list[at] = ((uint64_t)u << 32) | (uint32_t)~(from[i] + j);
+                        }
+                    }
+            }
+            __syncthreads();
+            ranked = found <= LP_ROOM;
+        }
+    }
+    if (ranked) {
+        const int held = found;
+        if (tid < held) {
+            const uint64_t mine = list[tid];
+            int rank = 0;
+            for (int i = 0; i < held; ++i) rank += list[i] > mine ? 1 : 0;
+            if (rank < top) {
+                const int id = (int)~(uint32_t)mine;
+                top_ids[(size_t)row * top + rank] = id;
+                top_logprob[(size_t)row * top + rank] = (float_of((uint32_t)(mine >> 32)) - m) - log_s;
+            }
+        }
+        return;
+    }
+    // the groups with the k first maxima, one after the other, then their logits
     uint64_t before = ~0ull;
-    for (int k = 0; k < top && k < groups; ++k) {
+    for (int k = 0; k < want; ++k) {
         uint64_t best = 0;
         for (int i = tid; i < groups; i += NT) {
-            const uint64_t key = ((uint64_t)order_of(tops[i]) << 32) | (uint32_t)~i;
+            const uint64_t key = ((uint64_t)keys[i] << 32) | (uint32_t)~i;
             if (key < before && key > best) best = key;
         }
         before = block_max64(best, red64);
         if (tid == 0) chosen[k] = (int)~(uint32_t)before;
     }
     __syncthreads();
-    const int n = (top < groups ? top : groups) * LP_GROUP;
+    uint32_t* logits = keys + groups;                     // these groups' logits, in their order; 0: behind the row's end
+    for (int i = tid; i < want * LP_GROUP; i += NT) {
+        const int e = chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP;
+        logits[i] = e < V ? order_of(src[e]) : 0u;
+    }
     before = ~0ull;
     for (int k = 0; k < top; ++k) {
         uint64_t best = 0;
-        for (int i = tid; i < n; i += NT) {
-            const int e = chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP;
-            if (e >= V) continue;
-            const uint64_t key = ((uint64_t)order_of(src[e]) << 32) | (uint32_t)~e;
-            if (key < before && key > best) best = key;
+        for (int i = tid; i < want * LP_GROUP; i += NT) {            // (a thread's own)
+            const uint64_t key = ((uint64_t)logits[i] << 32) | (uint32_t)~(chosen[i / LP_GROUP] * LP_GROUP + i % LP_GROUP);
+            if (logits[i] && key < before && key > best) best = key;
         }
         before = block_max64(best, red64);
         if (tid == 0) {
             const int id = (int)~(uint32_t)before;
             top_ids[(size_t)row * top + k] = id;
-            top_logprob[(size_t)row * top + k] = (src[id] - m) - log_s;
+            top_logprob[(size_t)row * top + k] = (float_of((uint32_t)(before >> 32)) - m) - log_s;
         }
     }
 }
@@ -199,6 +312,6 @@ extern "C" int li_token_logprobs(const float* logits, long stride, const int* id
         if (u == 2) logprob_rows_kernel<2><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
         else logprob_rows_kernel<8><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
     }
-    logprob_join_kernel<<<n, 64 * LP_WAVES, 0, stream>>>(logits, stride, V, shares, share, tops, groups, ids, logprob, entropy, top, top_ids, top_logprob);
+    logprob_join_kernel<<<n, 64 * LP_WAVES, top ? 4 * (groups + (top < groups ? top : groups) * LP_GROUP) : 0, stream>>>(logits, stride, V, shares, share, tops, groups, ids, logprob, entropy, top, top_ids, top_logprob);
     return li_launch_status();
 }

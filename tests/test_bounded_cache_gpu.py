@@ -198,6 +198,15 @@ def test_select_of_long_requests():
     check_select(mass, table, lens, keep, 4, 50, 30001)
 
 
+@pytest.mark.parametrize("longest", [1023, 1025, 4000, 4097, 16000, 16400, 32000, 33000])
+def test_select_of_every_length(longest):
+    """Each form of the kernel, with sums that are all different and sums of which many are equal."""
+    lens, keep = [longest, longest // 2, 3], [longest // 3, 5, 3]
+    table, mass, _, g = cache(lens, 1, 1, 16)
+    check_select(mass, table, lens, keep, 2, 9, longest // 3)
+    check_select(torch.floor(mass), table, lens, keep, 2, 9, longest // 3)
+
+
 @pytest.mark.parametrize("page_size", [16, 5])
 @pytest.mark.parametrize("shapes", [[(64, torch.bfloat16)] * 2 + [(1, torch.float32)], [(128, torch.float32)] * 2 + [(1, torch.float32)],
                                     [(36, torch.bfloat16), (2, torch.bfloat16)], [(256, torch.bfloat16)], [(3, torch.float32), (6, torch.bfloat16)] * 2])
