@@ -1173,61 +1173,97 @@ extern "C" int li_evict_select(const float* mass, const int* block_table, int ma
 
 // ------------------------------------------------------------------ the kept rows move to the front
 #define CMP_NT 256
-#define CMP_U 8
+#define CMP_U 4                   // pieces of a thread that move at a time
+#define CMP_LIST 2048             // rows whose addresses lie in LDS
 #define CMP_MAX_TENSORS 4
 
 struct CompactTensors {
     void* data[CMP_MAX_TENSORS];
     int pieces[CMP_MAX_TENSORS];         // pieces of a row
     int wide[CMP_MAX_TENSORS];           // a piece is 16 bytes, else 4
-    int count;
+    uint32_t inv[CMP_MAX_TENSORS];       // 2^32 / pieces
 };
 
 // kept is ascending, so kept[j] >= j: rows that are read lie at or behind those that are written, and rows of a later chunk behind
-// all that an earlier one writes.  A chunk is read whole, then written.
+// all that an earlier one writes.  So a chunk's rows may be asked for any time before, and have to have arrived, for all threads, before it is
+// written: the chunk behind is on its way while one waits at the barrier and is written.  Where a row stays, or has no page, nothing is written.
 template <typename V>
-__device__ __forceinline__ void compact_rows(V* __restrict__ data, int pieces, const int* __restrict__ kept, int K, const int* __restrict__ table,
-                                             int max_blocks, int kvh, int nkv, int page_size, int num_pages) {
+__device__ __forceinline__ void compact_rows(V* __restrict__ data, int pieces, uint32_t inv, const int* __restrict__ kept, int K, const int* __restrict__ table,
+                                             int max_blocks, int kvh, int nkv, int page_size, uint32_t page_inv, int num_pages,
+                                             int* from, int* to) {
+    const int tid = threadIdx.x;
     const long room = (long)max_blocks * page_size;
-    const long total = (long)K * pieces;
-    auto row_of = [&](int t) -> long {
-        const int page = table[t / page_size];
-        return page < 0 || page >= num_pages ? -1 : ((long)page * nkv + kvh) * page_size + t % page_size;
+    auto row_of = [&](int t) -> int {
+        int p = (int)__umulhi((uint32_t)t, page_inv), rest = t - p * page_size;
+        if (rest >= page_size) { ++p; rest -= page_size; }
+        const int page = table[p];
+        return page < 0 || page >= num_pages ? -1 : (page * nkv + kvh) * page_size + rest;
     };
-    for (long p0 = 0; p0 < total; p0 += CMP_NT * CMP_U) {
-        if (kept[p0 / pieces] < 0) break;                // (the list has ended: the same answer in every thread)
-        V v[CMP_U];
-        long to[CMP_U];
+    // a thread's pieces of a chunk of whole rows: row and piece of the row are the same in every chunk
+    const int rows = max(CMP_NT * CMP_U / pieces, 1), spread = rows * pieces;
+    int row[CMP_U], piece[CMP_U];
 #pragma unroll
-        for (int u = 0; u < CMP_U; ++u) {
-            const long p = p0 + threadIdx.x + (long)CMP_NT * u;
-            to[u] = -1;
-            if (p >= total) continue;
-            const int j = (int)(p / pieces), c = (int)(p % pieces), src = kept[j];
-            if (src <= j || src >= room) continue;       // the list's end, or a row that stays
-            const long a = row_of(src), b = row_of(j);
-            if (a < 0 || b < 0) continue;
-            v[u] = data[a * pieces + c];
-            to[u] = b * pieces + c;
+    for (int u = 0; u < CMP_U; ++u) {
+        const int p = tid + CMP_NT * u;
+        int r = (int)__umulhi((uint32_t)p, inv);
+        if (p - r * pieces >= pieces) ++r;
+        row[u] = p < spread ? r : CMP_LIST;               // (none)
+        piece[u] = p - r * pieces;
+    }
+    for (int j0 = 0; j0 < K; j0 += CMP_LIST) {
+        const int n = min(K - j0, CMP_LIST);
+        __syncthreads();
+        bool any = false;
+        for (int j = tid; j < n; j += CMP_NT) {
+            const int src = kept[j0 + j];
+            any |= src >= 0;
+            int a = -1, b = -1;
+            if (src > j0 + j && src < room) {             // (not the list's end, nor a row that stays)
+                a = row_of(src);
+                b = row_of(j0 + j);
+            }
+            from[j] = a < 0 || b < 0 ? -1 : a;
+            to[j] = b;
         }
-        __builtin_amdgcn_s_waitcnt(0);                   // what was asked for has arrived
-        __syncthreads();
+        if (!__syncthreads_or(any)) return;
+        V v[2][CMP_U];
+        auto load = [&](V (&x)[CMP_U], int first) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < CMP_U; ++u)
-            if (to[u] >= 0) data[to[u]] = v[u];
-        __syncthreads();
+            for (int u = 0; u < CMP_U; ++u) {
+                const int r = first + row[u], a = r < n ? from[r] : -1;
+                x[u] = data[(size_t)max(a, 0) * pieces + piece[u]];
+            }
+        };
+        auto store = [&](V (&x)[CMP_U], int first) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < CMP_U; ++u) asm volatile("" : "+v"(x[u]));       // what was asked for has arrived ...
+            __syncthreads();                                                     // ... for all threads
+#pragma unroll
+            for (int u = 0; u < CMP_U; ++u) {
+                const int r = first + row[u];
+                if (r < n && from[r] >= 0) data[(size_t)to[r] * pieces + piece[u]] = x[u];
+            }
+        };
+        load(v[0], 0);
+        for (int first = 0; first < n; first += 2 * rows) {
+            load(v[1], first + rows);
+            store(v[0], first);
+            load(v[0], first + 2 * rows);
+            store(v[1], first + rows);
+        }
     }
 }
 
-__global__ __launch_bounds__(CMP_NT) void cache_compact_kernel(CompactTensors ts, const int* __restrict__ kept, int K, const int* __restrict__ block_table,
-                                                               int max_blocks, int n, int nkv, int page_size, int num_pages) {
+__global__ __launch_bounds__(CMP_NT, 6) void cache_compact_kernel(CompactTensors ts, const int* __restrict__ kept, int K, const int* __restrict__ block_table,
+                                                               int max_blocks, int n, int nkv, int page_size, uint32_t page_inv, int num_pages) {
+    __shared__ int from[CMP_LIST], to[CMP_LIST];
     const int kvh = blockIdx.x % nkv, which = blockIdx.x / nkv, req = blockIdx.y, entry = blockIdx.z;
     const int* list = kept + (((size_t)entry * n + req) * nkv + kvh) * K;
     const int* table = block_table + (size_t)req * max_blocks;
     const int pieces = ts.pieces[which];
     const size_t base = (size_t)entry * num_pages * nkv * page_size * pieces;
-    if (ts.wide[which]) compact_rows((f32x4_t*)ts.data[which] + base, pieces, list, K, table, max_blocks, kvh, nkv, page_size, num_pages);
-    else compact_rows((float*)ts.data[which] + base, pieces, list, K, table, max_blocks, kvh, nkv, page_size, num_pages);
+    if (ts.wide[which]) compact_rows((f32x4_t*)ts.data[which] + base, pieces, ts.inv[which], list, K, table, max_blocks, kvh, nkv, page_size, page_inv, num_pages, from, to);
+    else compact_rows((float*)ts.data[which] + base, pieces, ts.inv[which], list, K, table, max_blocks, kvh, nkv, page_size, page_inv, num_pages, from, to);
 }
 
 // tensors: `count` pointers to [entries, num_pages, nkv, page_size, row] with rows of row_bytes[i] (multiples of 4); kept
@@ -1238,13 +1274,14 @@ extern "C" int li_cache_compact(void* const* tensors, const int* row_bytes, int 
         page_size <= 0 || (long)max_blocks * page_size >= 1L << 31)
         return LI_ERR_SIZE;
     CompactTensors ts = {};
-    ts.count = count;
     for (int i = 0; i < count; ++i) {
         if (row_bytes[i] <= 0 || row_bytes[i] % 4) return LI_ERR_SIZE;
         ts.data[i] = tensors[i];
         ts.wide[i] = row_bytes[i] % 16 == 0 && (uintptr_t)tensors[i] % 16 == 0;
         ts.pieces[i] = row_bytes[i] / (ts.wide[i] ? 16 : 4);
+        if (ts.pieces[i] > CMP_NT * CMP_U || (long)num_pages * nkv * page_size >= 1L << 31) return LI_ERR_SIZE;
+        ts.inv[i] = inverse_of(ts.pieces[i]);
     }
-    cache_compact_kernel<<<dim3(nkv * count, n, entries), CMP_NT, 0, stream>>>(ts, kept, K, block_table, max_blocks, n, nkv, page_size, num_pages);
+    cache_compact_kernel<<<dim3(nkv * count, n, entries), CMP_NT, 0, stream>>>(ts, kept, K, block_table, max_blocks, n, nkv, page_size, inverse_of(page_size), num_pages);
     return li_launch_status();
 }
