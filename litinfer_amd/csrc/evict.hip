@@ -796,8 +796,8 @@ static bool allow_lds(K kernel, int bytes) {
 }
 
 template <typename T, int DHP>
-static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg,
-                             int tokens, float* work, hipStream_t stream) {
+static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, bool padded,
+                             int nseg, int tokens, float* work, hipStream_t stream) {
     constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1, KEYS = 32 * ST * PT_WAVES;
     constexpr int LDS_BYTES = PT_BUFS * 32 * stage_tiles(DHP * (int)sizeof(T)) * DHP * (int)sizeof(T);
     if (p.single) {
@@ -805,7 +805,7 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
             SegList list;
             list.n = 0;
             int n = p.single;
-            if (p.single < nseg) {                       // a mix: the single ones are named
+            if (p.single < nseg || (!padded && nseg <= EV_LIST)) {   // a mix, or few: they are named, and their lengths need no trip to memory
                 n = 0;
                 for (; i < nseg && n < EV_LIST; ++i)
                     if (b.q_len[i] == 1) {
@@ -864,11 +864,11 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
 }
 
 template <typename T>
-static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg, int tokens,
+static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, bool padded, int nseg, int tokens,
                        float* work, hipStream_t stream) {
-    if (p.tiled && a.dh <= 64) return launch_mass_tiled<T, 64>(q, k, mass, a, p, b, nseg, tokens, work, stream);
-    if (p.tiled && a.dh <= 128) return launch_mass_tiled<T, 128>(q, k, mass, a, p, b, nseg, tokens, work, stream);
-    if (p.tiled) return launch_mass_tiled<T, 256>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    if (p.tiled && a.dh <= 64) return launch_mass_tiled<T, 64>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
+    if (p.tiled && a.dh <= 128) return launch_mass_tiled<T, 128>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
+    if (p.tiled) return launch_mass_tiled<T, 256>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
     mass_rows_kernel<T><<<dim3(p.multi_q, a.nh, nseg), 64, 0, stream>>>(q, k, a, work);
     mass_keys_kernel<T><<<dim3((p.multi_ctx + 63) / 64, a.nkv, nseg), 256, 0, stream>>>(q, k, a, work, mass);
     return li_launch_status();
@@ -895,8 +895,8 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
     const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale, tokens, nh, (long)num_pages * nkv * page_size));
     if (!p.valid || p.floats > work_floats) return LI_ERR_SIZE;
     const Batch b = {h_q_start, h_q_len, h_ctx_len};
-    if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, nseg, tokens, work, stream);
-    return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, nseg, tokens, work, stream);
+    if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, padded_ctx > 0, nseg, tokens, work, stream);
+    return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, padded_ctx > 0, nseg, tokens, work, stream);
 }
 
 // ------------------------------------------------------------------ which keys stay

@@ -1943,10 +1943,15 @@ LOGPROBS_MAX_TOP = 32                  # alternatives a row
 LOGPROBS_MAX_VOCAB = 1 << 20
 
 
-def _one_device(what: str, *ts) -> None:
-    """The kernels run on the current device and stream: tensors of another one are refused."""
+def _here(what: str, *ts) -> None:
+    """The kernels run on the current device and stream: tensors on the host, or on another device, are refused."""
+    if not ts[0].is_cuda:
+        _gpu(*ts)
     here = _get_device() if _get_device is not None else torch.cuda.current_device()
-    _chk(all(t is None or t.device.index == here for t in ts), f"{what}: all tensors have to be on the current device, cuda:{here}")
+    for t in ts:
+        if t is not None and t.get_device() != here:
+            _gpu(*ts)
+            raise ValueError(f"{what}: all tensors have to be on the current device, cuda:{here}")
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, entropy: torch.Tensor,
@@ -1956,21 +1961,23 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tens
     tokens in falling order, the lower id first on ties.  Logits of -inf have no probability: log probability -inf, no share of the entropy.  An id
     outside the row gives NaN.  A row whose largest logit is not finite, or that holds a NaN, gives NaN throughout; its top ids are ordered with
     NaN as -inf."""
-    _gpu(logits, ids, logprobs, entropy, top_ids, top_logprobs)
-    _one_device("token_logprobs", logits, ids, logprobs, entropy, top_ids, top_logprobs)
+    _here("token_logprobs", logits, ids, logprobs, entropy, top_ids, top_logprobs)
     _chk(_rows_ok(logits) and logits.dtype is torch.float32, "token_logprobs: logits must be float32 rows [n, V]")
     n, v = logits.shape
-    _chk(ids.dtype is torch.int32 and ids.shape == (n,) and ids.is_contiguous(), "token_logprobs: ids must be int32 [n]")
-    for t in (logprobs, entropy):
-        _chk(t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous(), "token_logprobs: logprobs and entropy must be float32 [n]")
-    _chk((top_ids is None) == (top_logprobs is None), "token_logprobs: top_ids and top_logprobs go together")
+    for t, dt in ((ids, torch.int32), (logprobs, torch.float32), (entropy, torch.float32)):
+        _chk(t.dtype is dt and t.shape == (n,) and t.is_contiguous(), "token_logprobs: ids must be int32 [n], logprobs and entropy float32 [n]")
     top = 0
-    if top_ids is not None:
-        _chk(top_ids.dim() == 2 and top_ids.shape[0] == n and top_ids.dtype is torch.int32 and top_ids.is_contiguous() and top_logprobs.shape == top_ids.shape
+    if top_ids is None or top_logprobs is None:
+        _chk(top_ids is top_logprobs, "token_logprobs: top_ids and top_logprobs go together")
+    else:
+        shape = top_ids.shape
+        _chk(len(shape) == 2 and shape[0] == n and top_ids.dtype is torch.int32 and top_ids.is_contiguous() and top_logprobs.shape == shape
              and top_logprobs.dtype is torch.float32 and top_logprobs.is_contiguous(), "token_logprobs: top_ids int32 and top_logprobs float32 [n, k]")
-        top = top_ids.shape[1]
-        _chk(top <= min(LOGPROBS_MAX_TOP, v), f"token_logprobs: {top} alternatives of {v} tokens (at most {LOGPROBS_MAX_TOP})")
-    _chk(0 < v <= LOGPROBS_MAX_VOCAB, f"token_logprobs: rows of {v} logits (1 to {LOGPROBS_MAX_VOCAB})")
+        top = shape[1]
+        if top > LOGPROBS_MAX_TOP or top > v:
+            _chk(False, f"token_logprobs: {top} alternatives of {v} tokens (at most {LOGPROBS_MAX_TOP})")
+    if not 0 < v <= LOGPROBS_MAX_VOCAB:
+        _chk(False, f"token_logprobs: rows of {v} logits (1 to {LOGPROBS_MAX_VOCAB})")
     if n:
         work = _scratch.floats(_logprobs_work_floats(n, v), logits.device)
         _run("logprobs", "li_token_logprobs", logits.data_ptr(), logits.stride(0), ids.data_ptr(), n, v, top, logprobs.data_ptr(), entropy.data_ptr(),
@@ -1991,8 +1998,7 @@ def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta,
     `fresh` the sums of the keys that this step wrote begin at zero (whatever the pages held); an entry that reads another's keys adds to all.
     Sums are float32 in an order that depends on the batch alone.  `ws` lends the buffers."""
     bt = meta.block_table
-    _gpu(qkv, mass, k, bt)
-    _one_device("attention_mass", qkv, mass, k, bt)
+    _here("attention_mass", qkv, mass, k, bt)
     pages = k.shape[0]
     _chk(mass.dtype is torch.float32 and mass.shape == (pages, nkv, page_size, 1) and mass.is_contiguous(),
          "attention_mass: mass must be float32 [pages, kv_heads, page_size, 1]")
@@ -2018,7 +2024,7 @@ def _mass_plan(qkv, k, meta, nh: int, nkv: int, dh: int, page_size: int, scale: 
     _check_qkv(qkv, nh, dh)
     _check_cache(k, k, nkv, dh, page_size, qkv.dtype)
     t, bt, n = qkv.shape[0], meta.block_table, meta.num_segments
-    _one_device("attention_mass", meta.q_start, meta.q_len, meta.ctx_len)
+    _here("attention_mass", meta.q_start, meta.q_len, meta.ctx_len)
     _chk(t == meta.num_tokens, "attention_mass: batch metadata is of another batch")
     _chk(bt.dtype is torch.int32 and bt.shape == (n, meta.max_blocks) and bt.is_contiguous(), "attention_mass: block table")
     _chk(all(x.dtype is torch.int32 and x.numel() == n and x.is_contiguous() for x in (meta.q_start, meta.q_len, meta.ctx_len)),
@@ -2054,8 +2060,7 @@ def evict_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tens
     largest sums, the lower place first on ties (a sum of NaN after all others).  mass [entries, pages, kv_heads, page_size, 1] float32;
     block_table int32 [requests, blocks]; lens, keep int32 [requests]; out int32 [entries, requests, kv_heads, K]: the places in rising
     order, -1 behind the last."""
-    _gpu(mass, block_table, lens, keep, out)
-    _one_device("evict_select", mass, block_table, lens, keep, out)
+    _here("evict_select", mass, block_table, lens, keep, out)
     _chk(mass.dim() == 5 and mass.shape[4] == 1 and mass.dtype is torch.float32 and mass.is_contiguous(),
          "evict_select: mass must be float32 [entries, pages, kv_heads, page_size, 1]")
     entries, pages, nkv, page_size, _ = mass.shape
@@ -2081,8 +2086,7 @@ def cache_compact(tensors, block_table: torch.Tensor, kept: torch.Tensor) -> Non
     [entries, requests, kv_heads, K] in rising order, -1 behind the last (as `evict_select` leaves it).  A place beyond the table, or on a page
     that the table does not have, is not moved."""
     tensors = list(tensors)
-    _gpu(*tensors, block_table, kept)
-    _one_device("cache_compact", *tensors, block_table, kept)
+    _here("cache_compact", *tensors, block_table, kept)
     _chk(1 <= len(tensors) <= CACHE_COMPACT_MAX_TENSORS, f"cache_compact: 1 to {CACHE_COMPACT_MAX_TENSORS} tensors")
     _chk(kept.dim() == 4 and kept.dtype is torch.int32 and kept.is_contiguous(), "cache_compact: kept must be int32 [entries, requests, kv_heads, K]")
     entries, n, nkv, most = kept.shape
