@@ -444,10 +444,10 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     for (int x = 0; x < ST; ++x) { m[x] = -INFINITY; l[x] = 0.f; }
     // (the rows of a stage are looked up in the table a stage before they are asked for, one a lane)
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
-    int row = 0;
-    auto look_up = [&](int s) __attribute__((always_inline)) { row = (int)some_row(a, table, kvh, min(s * ROWS + lane % ROWS, last)) * pieces; };
+    uint32_t row = 0;                                    // in pieces
+    auto look_up = [&](int s) __attribute__((always_inline)) { row = (uint32_t)some_row(a, table, kvh, min(s * ROWS + lane % ROWS, last)) * pieces; };
     auto load = [&](int buf) __attribute__((always_inline)) {
-        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, k, pieces, w, lane, [&](int r) { return (uint32_t)__shfl(row, r, LI_WAVE); });
+        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, k, pieces, w, lane, [&](int r) { return (uint32_t)__shfl((int)row, r, LI_WAVE); });
     };
     int at[CH];
     staged_at<PPR>(c, half, at);

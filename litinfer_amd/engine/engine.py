@@ -64,7 +64,8 @@ class Engine:
         32-bit or half precision in 32-bit (their products then run in the 32-bit kernels) instead of
         rounding them once to bfloat16 when they are bound.
         attention_mass: keep, beside every cached key, the attention weight that it has drawn, so that `evict`
-        can cut a request's cache to the tokens that drew most (models whose every layer attends over all its keys and values)."""
+        can cut a request's cache to the tokens that drew most (models whose every layer attends over all its keys and values).
+        A step whose forward raises may have added to some layers' sums; the same tokens then count twice there."""
         self.spec = spec
         self.config = config
         self.rt = Runtime(torch.device(device), parse_dtype(dtype), bool(keep_stored_precision), attention_mass=bool(attention_mass))

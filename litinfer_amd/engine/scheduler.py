@@ -178,6 +178,8 @@ class Scheduler:
         """logprobs: keep every generated token's log probability and that many alternatives (0: none) in `Request.logprobs`: of
         the model's own distribution, before temperature and cuts."""
         logprobs = check_top(logprobs, self.engine.spec.vocab_size, "add_request")
+        if logprobs is not None and not hasattr(self.sampler, "logprobs_async"):
+            raise ValueError("add_request: the scheduler's sampler works out no log probabilities (`logprobs_async`)")
         prompt = [int(t) for t in prompt]
         if not prompt:
             raise ValueError("add_request: inputs must not be empty")

@@ -11,8 +11,7 @@ def no_gpu(monkeypatch):
     """The argument checks alone: tensors may lie on the host, and nothing may be launched."""
     def launched(*a, **k):
         raise AssertionError("a call that has to be refused was launched")
-    monkeypatch.setattr(ops, "_gpu", lambda *ts: None)
-    monkeypatch.setattr(ops, "_one_device", lambda what, *ts: None)
+    monkeypatch.setattr(ops, "_here", lambda what, *ts: None)
     monkeypatch.setattr(ops, "_run", launched)
 
 

@@ -229,6 +229,18 @@ def test_log_probabilities_of_generated_tokens(bounded_ops, model, lookahead):
             sched.add_request([1, 2], 2, logprobs=bad)
 
 
+def test_a_sampler_without_log_probabilities_is_refused_when_they_are_asked_for(bounded_ops, model):
+    class Own:
+        def sample(self, logits, params, counters):
+            return [0] * logits.shape[0]
+    sched = Scheduler(engine(model), sampler=Own())
+    with pytest.raises(ValueError, match="no log probabilities"):
+        sched.add_request([1, 2], 2, logprobs=0)
+    rid = sched.add_request([1, 2], 2)
+    sched.run_to_completion()
+    assert sched.output(rid) == [0, 0]
+
+
 def test_log_probabilities_of_a_preempted_request(bounded_ops, model):
     def run(**kw):
         sched = Scheduler(engine(model, **kw), chunk_size=16)

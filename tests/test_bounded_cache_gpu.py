@@ -121,6 +121,62 @@ def test_mass_of_infinite_and_undefined_keys(dtype):
     assert torch.isfinite(mass[meta.block_table[1].long()[t // 16], :, t % 16, 0]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mass_of_many_requests(dtype):
+    """More than a launch names one by one: single tokens alone, portions alone, both."""
+    check_mass([(1, 3 + 5 * i) for i in range(70)], 4, 2, 64, 16, dtype)
+    check_mass([(2 + i % 3, 9 + 3 * i) for i in range(70)], 4, 2, 64, 16, dtype)
+    check_mass([(1 if i % 2 else 2 + i % 5, 9 + 3 * i) for i in range(150)], 4, 2, 64, 16, dtype)
+    check_mass([(1, 600)] * 130, 4, 2, 64, 16, dtype)
+
+
+def test_operators_on_the_last_pages_of_a_large_pool():
+    """Keys whose place in the pool passes 2^31 elements, and 2^32 bytes."""
+    pages, nkv, dh = 300000, 4, 128
+    k = torch.zeros(1, pages, nkv, 16, dh, dtype=torch.bfloat16, device=DEV)
+    mass = torch.zeros(1, pages, nkv, 16, 1, device=DEV)
+    small, _ = cases.batch([(1, 400), (70, 300), (1, 30)], 16, DEV, 3)
+    g = torch.Generator().manual_seed(9)
+    used = int(small.block_table.max()) + 1
+    few_k, few_mass = torch.randn(1, used, nkv, 16, dh, generator=g).bfloat16().to(DEV), torch.rand(1, used, nkv, 16, 1, generator=g).to(DEV)
+    k[:, pages - used:], mass[:, pages - used:] = few_k, few_mass
+    qkv = torch.randn(72, 12 * dh + 2 * nkv * dh, generator=g).bfloat16().to(DEV)
+    far, _ = cases.batch([(1, 400), (70, 300), (1, 30)], 16, DEV, 3)
+    far.block_table = torch.where(far.block_table >= 0, far.block_table + (pages - used), -1).to(torch.int32)
+    lens, keep = ints([400, 300, 30]), ints([100, 90, 20])
+    out = []
+    for pool_k, pool_m, meta in ((few_k, few_mass, small), (k, mass, far)):
+        ops.attention_mass(qkv, pool_m[0], pool_k[0], meta, 12, nkv, dh, 16, dh ** -0.5)
+        kept = torch.empty(1, 3, nkv, 100, dtype=torch.int32, device=DEV)
+        ops.evict_select(pool_m, meta.block_table, lens, keep, 4, 20, kept)
+        ops.cache_compact([pool_k, pool_m], meta.block_table, kept)
+        out.append((kept, pool_k[:, -used:].clone(), pool_m[:, -used:].clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    assert not k[:, :pages - used].any() and not mass[:, :pages - used].any()
+
+
+def test_mass_of_a_batch_that_has_changed_since():
+    """What is looked at once a step is looked at again for other arrays, and a batch that has grown in place is refused."""
+    qkv, mass, k, meta = mass_inputs([(1, 50), (1, 600)], 4, 2, 64, 16, torch.bfloat16)
+    args = (4, 2, 64, 16, 0.125)
+    ops.attention_mass(qkv, mass, k, meta, *args)
+    other = mass_inputs([(1, 40), (1, 500)], 4, 2, 64, 16, torch.bfloat16)[3]
+    for name in ("q_start", "q_len", "ctx_len", "host_q_start", "host_q_len", "host_ctx_len"):
+        setattr(meta, name, getattr(other, name))
+    meta.max_ctx_len = other.max_ctx_len
+    want = cases.plain_mass(qkv, mass, k, meta, *args)
+    ops.attention_mass(qkv, mass, k, meta, *args)
+    assert torch.allclose(mass.cpu().double(), want, rtol=mass_tolerance(qkv, k, meta, 4, 2, 64, 0.125), atol=1e-30)
+    short = mass_inputs([(1, 5), (1, 600)], 4, 2, 64, 16, torch.bfloat16)
+    meta = short[3]
+    meta.block_table = torch.cat([meta.block_table, torch.full((2, 400), -1, dtype=torch.int32, device=DEV)], 1)
+    meta.max_blocks = meta.block_table.shape[1]
+    ops.attention_mass(short[0], short[1], short[2], meta, *args)
+    meta.host_ctx_len[0] = 6000
+    with pytest.raises(RuntimeError, match="refused"):
+        ops.attention_mass(short[0], short[1], short[2], meta, *args)
+
+
 def test_mass_in_a_recording_and_on_another_stream():
     qkv, mass, k, meta = mass_inputs([(1, 130), (1, 260), (1, 33)], 12, 2, 128, 16, torch.bfloat16)
     want = mass.clone()
