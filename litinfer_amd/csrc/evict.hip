@@ -11,6 +11,7 @@
 // place / page size to the page.
 #include "common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #define EV_MAX_DH 256
@@ -394,21 +395,14 @@ __device__ __forceinline__ void in_steps(int n, Step step) {
     }
 }
 
-// Whether every place of 0 .. n - 1 has a page (the same answer in every thread of the block).
-__device__ __forceinline__ bool all_there(const MassArgs& a, const int* table, int n) {
-    const int blocks = (n + a.page_size - 1) / a.page_size;
-    int bad = 0;
-    for (int i = threadIdx.x; i < blocks; i += blockDim.x) bad |= table[i] < 0 || table[i] >= a.num_pages;
-    return !__syncthreads_or(bad);
-}
-
 // The rows' statistics: a wave holds ST * 32 queries of one head, the block streams keys.  Wave tiles of a kv head are numbered from the
-// last queries, whose rows are the longest, to the first, a tile's heads side by side: the four that a block takes see about the same keys.  grid: x kv heads times wave tiles / 4 (of the longest segment), z segments * splits of the keys.  The kv head
+// last queries, whose rows are the longest, to the first, a tile's heads side by side: the four that a block takes see about the same keys.  grid: x kv heads times wave tiles / 4 (of the longest segment), z segments * splits; a split is `share` stages of keys.  The kv head
 // goes fastest, here and below: blocks go round the XCDs, so an XCD's second-level cache holds one kv head's rows, or a few.
-// stats [splits, T, nh], or, where there is one split, lse [T, nh] itself.
+// stats [splits, nh, T], or, where there is one split, lse [nh, T] itself.
 template <typename T, int DHP, int ST>
 __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                       float2* __restrict__ stats, float* __restrict__ lse, int splits, int tokens) {
+                                                                       float2* __restrict__ stats, float* __restrict__ lse, int splits, int share,
+                                                                       int tokens) {
     constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int which = blockIdx.z / splits, seg = list.seg[which], split = blockIdx.z % splits, kvh = blockIdx.x % a.nkv, tok0 = list.start[which];
@@ -422,8 +416,12 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     const int h = kvh * rep + wt % rep, i0 = (tiles - 1 - wt / rep) * (32 * ST);
     // the block's keys: up to the last that its first wave sees, this split's share of the stages
     const int last = base + min((tiles - wt0 / rep) * (32 * ST), nq) - 1;
-    const int stages = last / ROWS + 1, s0 = (int)((long)stages * split / splits), s1 = (int)((long)stages * (split + 1) / splits);
-    const bool whole = all_there(a, table, last + 1);
+    const int s0 = split * share, s1 = min(last / ROWS + 1, s0 + share);
+    if (s0 >= s1) {                                      // none (and there is another split): nothing is what its rows add
+        for (int i = i0 + lane; mine && i < min(i0 + 32 * ST, nq); i += 64)
+            stats[((size_t)split * a.nh + h) * tokens + tok0 + i] = make_float2(-INFINITY, 0.f);
+        return;
+    }
     if (pieces < PPR) {
         for (int i = tid; i < PT_BUFS * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
         __syncthreads();
@@ -445,8 +443,15 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     // (the rows of a stage are looked up in the table a stage before they are asked for, one a lane)
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
     uint32_t row = 0;                                    // in pieces
-    auto look_up = [&](int s) __attribute__((always_inline)) { row = (uint32_t)some_row(a, table, kvh, min(s * ROWS + lane % ROWS, last)) * pieces; };
-    auto load = [&](int buf) __attribute__((always_inline)) {
+    uint64_t next_there = 0, there[PT_BUFS];             // which of a stage's keys have a page
+    auto look_up = [&](int s) __attribute__((always_inline)) {
+        const long r = place_row(a, table, kvh, min(s * ROWS + lane % ROWS, last));
+        next_there = __ballot(r >= 0);
+        row = (uint32_t)(r < 0 ? (long)kvh * a.page_size : r) * pieces;
+    };
+    auto load = [&](auto which_buf) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which_buf)::value;
+        there[buf] = next_there;
         stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, k, pieces, w, lane, [&](int r) { return (uint32_t)__shfl((int)row, r, LI_WAVE); });
     };
     int at[CH];
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     // A tile joins the rows' statistics in CH shares: the first quarter finds the maxima, the others add up.
     float b[ST], sum[ST];
     constexpr int LEAD = CH / 4, EACH = CH - LEAD;
-    auto share = [&](const f32x16_t (&acc)[ST], int j) __attribute__((always_inline)) {
+    auto add_up = [&](const f32x16_t (&acc)[ST], int j) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < ST; ++x) {
             if (j == x * LEAD / ST) {
@@ -476,10 +481,8 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
         }
     };
     // keys that a query does not see, if there may be any among these 32
-    auto hide = [&](f32x16_t (&acc)[ST], int k0) __attribute__((always_inline)) {
-        if (whole && k0 + 31 <= seen_all) return;
-        uint32_t there = ~0u;
-        if (!whole) there = (uint32_t)__ballot(place_row(a, table, kvh, min(k0 + c, last)) >= 0);
+    auto hide = [&](f32x16_t (&acc)[ST], int k0, uint32_t there) __attribute__((always_inline)) {
+        if (there == ~0u && k0 + 31 <= seen_all) return;
         there >>= 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -496,39 +499,37 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     nothing<ST>(acc[0]);
     nothing<ST>(acc[1]);
     int pending = 0;
-    if (s0 < s1) {
-        look_up(s0);
-        load(0);
-        look_up(s0 + 1);
-        if (s0 + 1 < s1) {
-            load(1);
-            look_up(s0 + 2);
-            arrived<LOADS>();
-        } else {
-            arrived<0>();
-        }
-#pragma unroll
-        for (int j = 0; j < PT_RING; ++j) ring[j] = staged_piece(lds, at[j]);
+    look_up(s0);
+    load(std::integral_constant<int, 0>{});
+    look_up(s0 + 1);
+    if (s0 + 1 < s1) {
+        load(std::integral_constant<int, 1>{});
+        look_up(s0 + 2);
+        arrived<LOADS>();
+    } else {
+        arrived<0>();
     }
+#pragma unroll
+    for (int j = 0; j < PT_RING; ++j) ring[j] = staged_piece(lds, at[j]);
     in_steps((s1 - s0) * TPS, [&](auto index, int t) __attribute__((always_inline)) {
         constexpr int I = decltype(index)::value, buf = I / TPS % PT_BUFS, y = I % TPS, nbuf = (I + 1) / TPS % PT_BUFS, ny = (I + 1) % TPS, now = I & 1;
         const int s = s0 + t / TPS, k0 = s * ROWS + 32 * y;
         if (y == TPS - 1 && s + 1 < s1) {                // the next stage is there, and nobody reads the one before this any more
             arrived<0>();
-            if (s + 2 < s1) { load((buf + 2) % PT_BUFS); look_up(s + 3); }
+            if (s + 2 < s1) { load(std::integral_constant<int, (buf + 2) % PT_BUFS>{}); look_up(s + 3); }
         }
         if (k0 > seen_any) return;
         multiply_rows<CH, ST>(lds + buf * STAGE_BYTES + 32 * y * PPR * 16, lds + nbuf * STAGE_BYTES + 32 * ny * PPR * 16, at, ring, qf, acc[now],
                               [](const u32x4_t staged, const u32x4_t held, f32x16_t v) { return mma32<T>(staged, held, v); },
-                              [&](int j) __attribute__((always_inline)) { share(acc[now ^ 1], j); });
+                              [&](int j) __attribute__((always_inline)) { add_up(acc[now ^ 1], j); });
         stay();
-        hide(acc[now], k0);
+        hide(acc[now], k0, (uint32_t)(there[buf] >> (32 * y)));
         pending = now;
     });
 #pragma unroll
     for (int j = 0; j < CH; ++j) {                       // the last tile's
-        if (pending == 0) share(acc[0], j);
-        else share(acc[1], j);
+        if (pending == 0) add_up(acc[0], j);
+        else add_up(acc[1], j);
     }
 #pragma unroll
     for (int x = 0; x < ST; ++x) {
@@ -536,13 +537,13 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
         const float sum = lane_xor_add(l[x] * __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b), 32);
         const int i = i0 + 32 * x + c;
         if (!mine || half != 0 || i >= nq) continue;
-        const size_t at = (size_t)(tok0 + i) * a.nh + h;
+        const size_t at = (size_t)h * tokens + tok0 + i;
         if (splits > 1) stats[(size_t)split * tokens * a.nh + at] = make_float2(mx, sum);
         else lse[at] = sum == 0.f ? INFINITY : (mx == -INFINITY ? 0.f : mx) + log2f(sum);
     }
 }
 
-// lse [T, nh] from the splits' statistics (rows of other segments hold what they hold and are not asked for).
+// lse [nh, T] from the splits' statistics (rows of other segments hold what they hold and are not asked for).
 __global__ __launch_bounds__(256) void mass_lse_kernel(const float2* __restrict__ stats, int splits, long rows, float* __restrict__ lse) {
     const long i = blockIdx.x * 256L + threadIdx.x;
     if (i >= rows) return;
@@ -557,11 +558,19 @@ __global__ __launch_bounds__(256) void mass_lse_kernel(const float2* __restrict_
 }
 
 // The columns' sums: a wave holds ST * 32 keys, the block streams the queries that see any of them, head by head.
-// grid: x kv heads times blocks of keys (of the longest segment), y splits of the (head, stage of queries) pairs, z segments.
+// grid: x kv heads times blocks of keys (of the longest segment), y splits of the (head, stage of queries) pairs, z segments.  A block of keys has
+// as many splits as make about `share` pairs each: late keys are seen by few queries.
 // part [splits, kv heads, places]; a segment's places begin at list.off.
+// The pairs of the block of keys from b0 on: its first stage of queries, stages a head, splits.
+struct Pairs { int first, n, splits; };
+__device__ __forceinline__ Pairs pairs_of(int b0, int base, int nq, int rep, int rows, int share) {
+    const int first = max(b0 - base, 0) / rows, n = (nq + rows - 1) / rows - first;
+    return {first, n, (rep * n + share - 1) / share};
+}
+
 template <typename T, int DHP, int ST>
 __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                       const float* __restrict__ lse, float* __restrict__ part, int splits, long places) {
+                                                                       const float* __restrict__ lse, float* __restrict__ part, int share, int tokens, long places) {
     constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16, KEYS = 32 * ST;
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -570,6 +579,8 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
     const int nq = list.q[which], ctx = list.ctx[which], base = ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE, tok0 = list.start[which];
     const int b0 = blockIdx.x / a.nkv * KEYS * PT_WAVES, k0 = b0 + w * KEYS;
     if (b0 >= ctx) return;
+    const Pairs pairs = pairs_of(b0, base, nq, rep, ROWS, share);
+    if (split >= pairs.splits) return;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
     if (pieces < PPR) {
         for (int i = tid; i < PT_BUFS * STAGE_BYTES / 16; i += 64 * PT_WAVES) reinterpret_cast<u32x4_t*>(lds)[i] = u32x4_t{0, 0, 0, 0};
@@ -588,8 +599,8 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
 #pragma unroll
         for (int r = 0; r < 16; ++r) sums[x][r] = 0.f;
     // pairs (head, stage of queries), numbered head by head; this split's share of them
-    const int first = max(b0 - base, 0) / ROWS, n = (nq + ROWS - 1) / ROWS - first;
-    const int u0 = (int)((long)rep * n * split / splits), u1 = (int)((long)rep * n * (split + 1) / splits);
+    const int first = pairs.first, n = pairs.n;
+    const int u0 = (int)((long)rep * n * split / pairs.splits), u1 = (int)((long)rep * n * (split + 1) / pairs.splits);
     int lh = u0 / n, ls = first + u0 % n;                // the pair that is loaded next
     const uint32_t q_pieces = a.q_row_stride / PE;
     float lq[PT_BUFS][TPS];                              // the queries' lse of the stages on their way, and where these begin
@@ -601,7 +612,7 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
 #pragma unroll
         for (int y = 0; y < TPS; ++y) {
             const int i = i0 + 32 * y + c;
-            lq[buf][y] = i < nq ? lse[(tok0 + i) * a.nh + kvh * rep + lh] : INFINITY;
+            lq[buf][y] = i < nq ? lse[(kvh * rep + lh) * tokens + tok0 + i] : INFINITY;
         }
         stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, q, pieces, w, lane, [&](int r) {
             return (uint32_t)(tok0 + min(i0 + r, nq - 1)) * q_pieces + (kvh * rep + lh) * pieces;
@@ -611,7 +622,7 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
     int at[CH];
     staged_at<PPR>(c, half, at);
     u32x4_t ring[PT_RING];
-    auto share = [&](const f32x16_t (&acc)[ST], float lq, int j) __attribute__((always_inline)) {       // a tile's sums, in CH shares
+    auto add_up = [&](const f32x16_t (&acc)[ST], float lq, int j) __attribute__((always_inline)) {       // a tile's sums, in CH shares
 #pragma unroll
         for (int x = 0; x < ST; ++x)
 #pragma unroll
@@ -662,15 +673,15 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
         }
         multiply_rows<CH, ST>(lds + buf * STAGE_BYTES + 32 * y * PPR * 16, lds + nbuf * STAGE_BYTES + 32 * ny * PPR * 16, at, ring, kf, acc[now],
                               [](const u32x4_t staged, const u32x4_t held, f32x16_t v) { return mma32<T>(held, staged, v); },
-                              [&](int j) __attribute__((always_inline)) { share(acc[now ^ 1], lacc[now ^ 1], j); });
+                              [&](int j) __attribute__((always_inline)) { add_up(acc[now ^ 1], lacc[now ^ 1], j); });
         stay();
         lacc[now] = lq[buf][y];
         hide(acc[now], lacc[now], from[buf] + 32 * y);
     });
 #pragma unroll
     for (int j = 0; j < CH; ++j) {                       // the last tile's
-        if (steps & 1) share(acc[0], lacc[0], j);
-        else share(acc[1], lacc[1], j);
+        if (steps & 1) add_up(acc[0], lacc[0], j);
+        else add_up(acc[1], lacc[1], j);
     }
     float* out = part + ((size_t)split * a.nkv + kvh) * places + list.off[blockIdx.z];
 #pragma unroll
@@ -685,12 +696,13 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
 }
 
 // The splits' sums, in their order, join the keys'.
-__global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list, const float* __restrict__ part, int splits, long places,
+__global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list, const float* __restrict__ part, int keys, int rows, int share, long places,
                                                         float* __restrict__ mass) {
     const int seg = list.seg[blockIdx.z], kvh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = list.ctx[blockIdx.z];
     if (t >= ctx) return;
     const long row = place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t);
     if (row < 0) return;
+    const int nq = list.q[blockIdx.z], splits = pairs_of(t / keys * keys, ctx - nq, nq, a.nh / a.nkv, rows, share).splits;
     const float* src = part + (size_t)kvh * places + list.off[blockIdx.z] + t;
     float sum = 0.f;
     for (int s = 0; s < splits; s += 4) {                // (four on their way at a time)
@@ -699,7 +711,7 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list
         for (int i = 0; i < 4; ++i) v[i] = s + i < splits ? src[(size_t)(s + i) * a.nkv * places] : 0.f;
         sum += (v[0] + v[1]) + (v[2] + v[3]);
     }
-    mass[row] = a.fresh && t >= ctx - list.q[blockIdx.z] ? sum : mass[row] + sum;
+    mass[row] = a.fresh && t >= ctx - nq ? sum : mass[row] + sum;
 }
 
 // ---- the plan of a batch, from its segments in host memory: which kernels, how many splits, where things lie in the workspace
@@ -709,7 +721,7 @@ struct MassPlan {
     long stride = 0;                     // keys of a head's scores
     int parts = 0, block_lds = 0;
     bool one_block = false;              // short contexts of single tokens: one kernel
-    int row_splits = 1, key_splits = 1, row_st = 1;
+    int row_splits = 1, key_splits = 1, row_st = 1, row_share = 1, key_share = 1, stage = 64;      // (shares: stages, pairs)
     long places = 0;                     // of the longer segments' sums, all together
     long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
     bool tiled = false, valid = false;
@@ -725,7 +737,7 @@ static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, cons
 
 static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, bool f32, bool tiled) {
     MassPlan p;
-    long total = 0, pairs = 0;
+    long total = 0;
     const int keys = 32 * PT_WAVES * (f32 ? 1 : 2);
     for (int i = 0; i < nseg; ++i) {
         const int ctx = padded_ctx > 0 ? padded_ctx : ctx_len[i];
@@ -739,7 +751,6 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
             p.multi_ctx = ctx > p.multi_ctx ? ctx : p.multi_ctx;
             p.multi_q = q_len[i] > p.multi_q ? q_len[i] : p.multi_q;
             p.places += (ctx + keys - 1) / keys * (long)keys;
-            pairs += (ctx + keys - 1) / keys;
         }
     }
     if (total != tokens || p.places >= 1L << 31) return p;
@@ -761,18 +772,36 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
         p.floats = p.one_block ? 0 : p.stats + 2L * p.single * nh * p.parts;
     }
     if (p.multi) {
-        // Blocks enough for some rounds over the compute units (two a unit at a time), each long enough to be worth its start: 1,999 queries of 40
-        // heads behind 16,000 keys, rows / columns at 512, 1,024 and 1,536 blocks 534, 478, 484 / 483, 440, 428 us.
-        // Rows: a wave holds two tiles of queries where that leaves two blocks a unit, else one (2,048 queries of 28 heads 37 us, with two 44;
-        // 1,999 behind 16,000 520 and 478).
-        const int stages = (p.multi_ctx + 63) / 64;
+        // Blocks of about equal length: as many as the compute units hold at a time, each with no less than 8 stages of keys (4 pairs of a head and a stage
+        // of queries), or, where there is work for many rounds, 96 stages (40 pairs) each.  Rows: a wave holds two tiles of queries where that
+        // leaves a whole round of such blocks.  A prompt of 2,048 of 28 heads on 4, us with least 4, 8, 12 and 16 pairs: 83, 88, 87, 81; 990 tokens of 12
+        // heads on 2 behind 500: 37, 40, 48, 51; 512 of 28 heads behind 4,000: 60, 65, 69, 74; 1,999 of 40 heads behind 16,000: 750 with all.
+        const int rows = 32 * stage_tiles((dh <= 64 ? 64 : dh <= 128 ? 128 : 256) * (f32 ? 4 : 2));
         for (p.row_st = f32 ? 1 : 2;; p.row_st = 1) {
-            const long blocks = ((long)(p.multi_q + 32 * p.row_st - 1) / (32 * p.row_st) * rep + PT_WAVES - 1) / PT_WAVES * nkv * p.multi;
-            for (p.row_splits = 1; p.row_splits < 16 && blocks * p.row_splits < 1024 && stages / (2 * p.row_splits) >= 8;) p.row_splits *= 2;
-            if (p.row_st == 1 || blocks * p.row_splits >= 512) break;
+            long stages = 0, most = 0;
+            for (int i = 0; i < nseg; ++i) {
+                if (q_len[i] < 2) continue;
+                const long tiles = (q_len[i] + 32 * p.row_st - 1) / (32 * p.row_st), blocks = (tiles * rep + PT_WAVES - 1) / PT_WAVES;
+                stages += blocks * nkv * ((ctx_len[i] - q_len[i] / 2 + rows - 1) / rows);
+                most = std::max(most, (long)(ctx_len[i] + rows - 1) / rows);
+            }
+            const long one = p.row_st == 2 || f32 ? 512 : 768;
+            p.row_share = (int)std::min(std::max((stages + one - 1) / one, 8L), 96L);
+            p.row_share = (int)std::max((long)p.row_share, (most + 511) / 512);
+            p.row_splits = (int)((most + p.row_share - 1) / p.row_share);
+            if (p.row_st == 1 || stages >= one * 16) break;
         }
-        const long key_blocks = pairs * nkv, units = (long)rep * ((p.multi_q + 63) / 64);
-        while (p.key_splits < 16 && key_blocks * p.key_splits < 1536 && units / (2 * p.key_splits) >= 2) p.key_splits *= 2;
+        long units = 0;
+        for (int i = 0; i < nseg; ++i) {
+            if (q_len[i] < 2) continue;
+            const long n = (q_len[i] + rows - 1) / rows, base = ctx_len[i] - q_len[i];
+            units += (long)nkv * rep * (base / keys * n + ((ctx_len[i] + keys - 1) / keys - base / keys) * (n + 1) / 2);
+        }
+        p.key_share = (int)std::min(std::max((units + 511) / 512, 4L), 40L);
+        const long longest = (long)rep * ((p.multi_q + rows - 1) / rows);
+        p.key_share = (int)std::max((long)p.key_share, (longest + 32767) / 32768);
+        p.key_splits = (int)((longest + p.key_share - 1) / p.key_share);
+        p.stage = rows;
         p.rows = p.floats;
         p.lse = p.rows + 2L * p.row_splits * tokens * nh;
         p.sums = p.lse + (long)tokens * nh;
@@ -850,11 +879,11 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                 at += n;
                 if (pass == 0) {
                     rows<<<dim3((tiles * rep + PT_WAVES - 1) / PT_WAVES * a.nkv, 1, n * p.row_splits), 64 * PT_WAVES, LDS_BYTES, stream>>>(
-                        q, k, a, list, stats, lse, p.row_splits, tokens);
+                        q, k, a, list, stats, lse, p.row_splits, p.row_share, tokens);
                 } else {
                     keys<<<dim3((p.multi_ctx + KEYS - 1) / KEYS * a.nkv, p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
-                        q, k, a, list, lse, sums, p.key_splits, p.places);
-                    mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, p.key_splits, p.places, mass);
+                        q, k, a, list, lse, sums, p.key_share, tokens, p.places);
+                    mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, KEYS, p.stage, p.key_share, p.places, mass);
                 }
             }
             if (pass == 0 && p.row_splits > 1) mass_lse_kernel<<<(unsigned)((rows_n + 255) / 256), 256, 0, stream>>>(stats, p.row_splits, rows_n, lse);
