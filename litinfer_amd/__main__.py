@@ -26,6 +26,13 @@ import math
 import sys
 
 
+def _perplexity(logprob: float, tokens: int):
+    try:
+        return math.exp(-logprob / tokens) if tokens else None
+    except OverflowError:
+        return math.inf
+
+
 def _cmd_generate(a) -> int:
     from .models import load
     if getattr(a, "test", False):
@@ -72,7 +79,7 @@ def _generate(a, load) -> int:
     if a.cmd == "score":
         rows = model.score(ids, top=a.top)
         total = sum(r.logprob for r in rows)
-        print(json.dumps({"tokens": len(rows), "logprob": total, "perplexity": math.exp(-total / len(rows)) if rows else None,
+        print(json.dumps({"tokens": len(rows), "logprob": total, "perplexity": _perplexity(total, len(rows)),
                           "rows": [{"token": r.token, "logprob": r.logprob, "entropy": r.entropy, "top": [list(t) for t in r.top]} for r in rows]}))
         return 0
     tokens, metrics = model.generate_profile(ids, max_new_tokens=a.max_steps, top_k=a.top_k,

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64) void mass_rows_kernel(const T* __restrict__ q, 
     __shared__ float qs[EV_MAX_DH];
     const int seg = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x;
     if (i >= a.q_len[seg]) return;
-    const int tok = a.q_start[seg] + i, seen = a.ctx_len[seg] - a.q_len[seg] + i + 1;
+    const int tok = a.q_start[seg] + i, seen = min(a.ctx_len[seg], a.max_blocks * a.page_size) - a.q_len[seg] + i + 1;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
     for (int d = lane; d < a.dh; d += 64) qs[d] = load_as_float(q + (size_t)tok * a.q_row_stride + (size_t)h * a.dh + d);
     __syncthreads();
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void mass_keys_kernel(const T* __restrict__ q,
                                                         float* __restrict__ mass) {
     __shared__ float qs[4][EV_MAX_DH], part[4][64];
     const int seg = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int nq = a.q_len[seg], ctx = a.ctx_len[seg], t = blockIdx.x * 64 + lane, rep = a.nh / a.nkv;
+    const int nq = a.q_len[seg], ctx = min(a.ctx_len[seg], a.max_blocks * a.page_size), t = blockIdx.x * 64 + lane, rep = a.nh / a.nkv;
     if ((int)blockIdx.x * 64 >= ctx) return;
     const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
     const int base = ctx - nq;                           // place of the step's first token
@@ -942,6 +942,7 @@ struct SelectArgs {
     int max_blocks, first, recent, K, nkv, page_size, num_pages;
     uint32_t page_inv;
     int* out;
+    int fours;                   // four places side by side lie in one page, on 16 bytes
 };
 
 // Places lo .. hi - 1 of a request compete for `want` of its places; the others of its `len` stay anyway.
@@ -1012,7 +1013,7 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(SelectArgs a) {
         uint32_t key[VPT];                                // 1 + the order of the sums that compete, 0 for the other places
         float sum[VPT];
         const int last = c.len - 1;
-        if (a.page_size % 4 == 0) {                       // four places of a page at a time
+        if (a.fours) {
             int at[VPT / 4];
 #pragma unroll
             for (int j = 0; j < VPT / 4; ++j) at[j] = table[page_of(a, min(t0 + 4 * j, last))];
@@ -1189,7 +1190,8 @@ extern "C" int li_evict_select(const float* mass, const int* block_table, int ma
     if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || first < 0 || recent < 0 || max_blocks <= 0 || num_pages <= 0 || page_size <= 0 ||
         (long)max_blocks * page_size >= 1L << 31)
         return LI_ERR_SIZE;
-    const SelectArgs a = {mass, block_table, lens, keeps, max_blocks, first, recent, K, nkv, page_size, num_pages, inverse_of(page_size), out};
+    const SelectArgs a = {mass, block_table, lens, keeps, max_blocks, first, recent, K, nkv, page_size, num_pages, inverse_of(page_size), out,
+                          page_size % 4 == 0 && (uintptr_t)mass % 16 == 0};
     const long room = (long)max_blocks * page_size;      // (as long as any request can be; the tables say no more)
     const dim3 grid(nkv, n, entries);
     if (room <= 1024) evict_select_kernel<256, 4><<<grid, 256, 0, stream>>>(a);
@@ -1300,7 +1302,7 @@ __global__ __launch_bounds__(CMP_NT, 6) void cache_compact_kernel(CompactTensors
 extern "C" int li_cache_compact(void* const* tensors, const int* row_bytes, int count, const int* block_table, int max_blocks, const int* kept, int K, int n,
                                 int entries, int nkv, int page_size, int num_pages, hipStream_t stream) {
     if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || count <= 0 || count > CMP_MAX_TENSORS || max_blocks <= 0 ||
-        page_size <= 0 || (long)max_blocks * page_size >= 1L << 31)
+        num_pages <= 0 || page_size <= 0 || (long)max_blocks * page_size >= 1L << 31)
         return LI_ERR_SIZE;
     CompactTensors ts = {};
     for (int i = 0; i < count; ++i) {

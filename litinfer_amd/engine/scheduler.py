@@ -147,9 +147,9 @@ class Scheduler:
             row_tile = int(getattr(engine, "row_tile", 1) or 1)
         if max_batch_tokens <= 0 or chunk_size <= 0 or row_tile <= 0:
             raise ValueError("scheduler: max_batch_tokens, chunk_size and row_tile must be positive")
-        if cache_budget is not None and (cache_budget <= 0 or cache_slack < 0 or not engine.rt.attention_mass):
-            raise ValueError("scheduler: a cache_budget is positive, its slack not negative, and the engine keeps attention weights "
-                             "(Engine(..., attention_mass=True))")
+        if cache_budget is not None and (cache_budget <= 0 or min(cache_slack, cache_first, cache_recent or 0) < 0 or not engine.rt.attention_mass):
+            raise ValueError("scheduler: a cache_budget is positive, cache_slack, cache_first and cache_recent are not negative, and the engine "
+                             "keeps attention weights (Engine(..., attention_mass=True))")
         self.engine = engine
         self.cache = engine.cache
         self.cache_budget = None if cache_budget is None else int(cache_budget)
@@ -178,7 +178,7 @@ class Scheduler:
         """logprobs: keep every generated token's log probability and that many alternatives (0: none) in `Request.logprobs`: of
         the model's own distribution, before temperature and cuts."""
         logprobs = check_top(logprobs, self.engine.spec.vocab_size, "add_request")
-        if logprobs is not None and not hasattr(self.sampler, "logprobs_async"):
+        if logprobs is not None and not (hasattr(self.sampler, "logprobs_async") and hasattr(self.sampler, "sample_async")):
             raise ValueError("add_request: the scheduler's sampler works out no log probabilities (`logprobs_async`)")
         prompt = [int(t) for t in prompt]
         if not prompt:

@@ -138,8 +138,9 @@ class CausalLM:
         sched, engine, rid = Scheduler(self.engine, **self._sched_args), self.engine, object()
         pending, given = [], torch.tensor(tokens[1:], dtype=torch.int32).to(engine.rt.device)
         try:
-            for at in range(0, len(given), sched.chunk_size):
-                part = tokens[at:min(at + sched.chunk_size, len(given))]
+            portion = min(sched.chunk_size, sched.max_batch_tokens)
+            for at in range(0, len(given), portion):
+                part = tokens[at:min(at + portion, len(given))]
                 logits = engine.step([StepEntry(rid, part, range(len(part)))])
                 pending.append(sched.sampler.logprobs_async(logits, given[at:at + len(part)], top))
                 sched.keep_within_budget([rid])

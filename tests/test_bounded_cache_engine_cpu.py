@@ -314,3 +314,24 @@ def test_score_on_the_command_line(bounded_ops, model, capsys):
     assert main(["generate", "--model", str(model), "--device", "cpu", "--dtype", "float32", "--num-pages", "40", "--prompt-ids", ",".join(map(str, text(200))), "--max_steps", "3",
                  "--test", "--cache-budget", "50"]) == 0
     assert len(json.loads(capsys.readouterr().out.splitlines()[-1])["tokens"]) == 3
+
+
+def test_a_perplexity_beyond_all_numbers():
+    from litinfer_amd.__main__ import _perplexity
+    assert _perplexity(-math.log(8.0) * 5, 5) == pytest.approx(8.0, rel=1e-12)
+    assert _perplexity(-1e5, 3) == math.inf and _perplexity(-math.inf, 3) == math.inf and _perplexity(0.0, 0) is None
+    assert math.isnan(_perplexity(math.nan, 2))
+
+
+def test_score_goes_by_the_largest_step(bounded_ops, model):
+    m = Qwen2(model, device="cpu", dtype="float32", page_size=8, max_tokens=256, max_seqs=2, chunk_size=64, max_batch_tokens=24)
+    sizes, step = [], m.engine.step
+    m.engine.step = lambda entries: sizes.append(sum(len(e.tokens) for e in entries)) or step(entries)
+    rows = m.score(text(71))
+    assert len(rows) == 70 and sizes == [24, 24, 22]
+
+
+@pytest.mark.parametrize("bad", [dict(cache_budget=0), dict(cache_slack=-1), dict(cache_first=-1), dict(cache_recent=-2)])
+def test_a_scheduler_refuses_budgets_that_make_no_sense(bounded_ops, model, bad):
+    with pytest.raises(ValueError, match="cache_budget"):
+        Scheduler(engine(model), **{"cache_budget": 16, **bad})

@@ -263,6 +263,16 @@ def test_select_of_every_length(longest):
     check_select(torch.floor(mass), table, lens, keep, 2, 9, longest // 3)
 
 
+@pytest.mark.parametrize("longest", [300, 3000, 9000])
+def test_select_of_sums_that_do_not_begin_on_16_bytes(longest):
+    lens, keep = [longest, longest - 7, 30], [longest // 2, 9, 30]
+    table, mass, _, _ = cache(lens, 2, 2, 16)
+    for off in (1, 2, 3):
+        view = torch.full((mass.numel() + off,), 1e9, device=DEV)[off:].view(mass.shape)
+        view.copy_(mass)
+        check_select(view, table, lens, keep, 3, 10, longest // 2)
+
+
 @pytest.mark.parametrize("page_size", [16, 5])
 @pytest.mark.parametrize("shapes", [[(64, torch.bfloat16)] * 2 + [(1, torch.float32)], [(128, torch.float32)] * 2 + [(1, torch.float32)],
                                     [(36, torch.bfloat16), (2, torch.bfloat16)], [(256, torch.bfloat16)], [(3, torch.float32), (6, torch.bfloat16)] * 2])
