@@ -5,8 +5,9 @@
 // The maximum's own share is counted, not added up, so that what is small beside it (the entropy of a sure row, the
 // log probability of its token) keeps its digits.  All sums are float32 with a fixed order.
 //
-// Bound by the one read of the logits.  A wave takes LP_GROUP * U of a row's logits into registers, finds their maximum and
-// then adds up against it: no running rescaling, one pass.  It also leaves the maximum of every group of LP_GROUP logits:
+// Bound by the one read of the logits (2,047 rows of 151,936: 1.24 GB in 212 us, 5.9 TB/s; 64 rows 12 us, of which 5 are the launches and the first trip to
+// memory; one row 4.6 us; 20 alternatives of each cost 27, 7.5 and 4 us more).  A wave takes LP_GROUP * U of a row's logits into registers, finds their
+// maximum and then adds up against it: no running rescaling, one pass.  It also leaves the maximum of every group of LP_GROUP logits:
 // the row's k largest logits, ordered by (value, lower index first), all lie in the k groups whose maxima are first in that
 // order (a group in front of them has a logit that is before any of theirs), so the second kernel reads k groups again
 // instead of the row.
@@ -16,6 +17,7 @@
 #define LP_MAX_GROUPS 4096
 #define LP_MAX_TOP 32
 #define LP_WAVES 4
+#define LP_JOIN_WAVES 8          // of a block that joins a row
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));        // (rows need not begin on 16 bytes)
 
@@ -62,9 +64,10 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_rows_kernel(const float
             const float g = wave_max(a);
             const int k = part * U + u;
             if (lane == 0 && k < groups) tops[(size_t)row * groups + k] = g;
+            m = fmaxf(m, g);
         }
     }
-    m = wave_max(m);
+    if (!tops) m = wave_max(m);
     const float base = m == -INFINITY ? 0.f : m;
     float c = 0.f, r = 0.f, t = 0.f;
 #pragma unroll
@@ -101,35 +104,39 @@ __device__ __forceinline__ uint64_t block_max64(uint64_t v, uint64_t* smem) {
     __syncthreads();
     uint64_t b = smem[0];
 #pragma unroll
-    for (int w = 1; w < LP_WAVES; ++w) b = smem[w] > b ? smem[w] : b;
+    for (int w = 1; w < LP_JOIN_WAVES; ++w) b = smem[w] > b ? smem[w] : b;
     return b;
 }
 
 // How many of the block's threads' values are counted by f, in every thread; `turn` alternates between calls (one barrier each).
 template <typename F>
-__device__ __forceinline__ int block_count(int n, int (*smem)[LP_WAVES], int turn, F f) {
+__device__ __forceinline__ int block_count(int n, int (*smem)[LP_JOIN_WAVES], int turn, F f) {
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += 64 * LP_WAVES) c += __popcll(__ballot(f(i)));      // (of the lanes that are still in the loop)
+    for (int i = threadIdx.x; i < n; i += 64 * LP_JOIN_WAVES) c += __popcll(__ballot(f(i)));      // (of the lanes that are still in the loop)
     if ((threadIdx.x & 63) == 0) smem[turn & 1][threadIdx.x >> 6] = c;       // (the wave's first lane leaves the loop last)
     __syncthreads();
-    return smem[turn & 1][0] + smem[turn & 1][1] + smem[turn & 1][2] + smem[turn & 1][3];
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < LP_JOIN_WAVES; ++w) c += smem[turn & 1][w];
+    return c;
 }
 
 // One block a row: joins the waves' shares, then finds the likeliest tokens.  A value that at least k and at most LP_LIST groups' maxima
 // reach is found by halving the range between the least and the largest; the logits of these groups that reach it are gathered (at least
 // k, seldom many more) and each one's rank counted.  Where many values are equal or likely tokens lie side by side no such value may exist, or more
-// logits reach it than there is room for: then the k first are taken one after the other.
+// logits reach it than there is room for: then the k first are taken one after the other.  A chain of short steps with a barrier behind each: eight waves
+// take 9.2 us for a row with 20 alternatives (both kernels), four 11.3, sixteen 9.0; at 2,047 rows 242, 242 and 256.
 #define LP_LIST 64                // groups that are looked through
 #define LP_ROOM 256               // logits that are ranked
-__global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float* __restrict__ x, long stride, int V, int shares,
+__global__ __launch_bounds__(64 * LP_JOIN_WAVES) void logprob_join_kernel(const float* __restrict__ x, long stride, int V, int shares,
                                                                      const RowShare* __restrict__ in, const float* __restrict__ tops, int groups,
                                                                      const int* __restrict__ ids, float* __restrict__ logprob,
                                                                      float* __restrict__ entropy, int top, int* __restrict__ top_ids,
                                                                      float* __restrict__ top_logprob) {
-    constexpr int NT = 64 * LP_WAVES;
-    __shared__ float red[LP_WAVES], sums[LP_WAVES][3];
-    __shared__ uint64_t red64[LP_WAVES], list[LP_ROOM];
-    __shared__ int chosen[LP_LIST], counts[2][LP_WAVES], found;
+    constexpr int NT = 64 * LP_JOIN_WAVES;
+    __shared__ float red[LP_JOIN_WAVES], sums[LP_JOIN_WAVES][3];
+    __shared__ uint64_t red64[LP_JOIN_WAVES], list[LP_ROOM];
+    __shared__ int chosen[LP_LIST], counts[2][LP_JOIN_WAVES], found;
     extern __shared__ uint32_t keys[];                    // the groups' maxima, in their order (and room for the k first groups' logits)
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const float* src = x + (size_t)row * stride;
@@ -148,7 +155,8 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float
     m = wave_max(m);
     if (lane == 0) red[w] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < LP_JOIN_WAVES; ++i) m = fmaxf(m, red[i]);
     float c = 0.f, r = 0.f, t = 0.f;
     for (int i = tid; i < shares; i += NT) {
         const RowShare s = i == tid ? first : in[i];
@@ -162,9 +170,9 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float
     t = wave_sum(t);
     if (lane == 0) { sums[w][0] = c; sums[w][1] = r; sums[w][2] = t; }
     __syncthreads();
-    c = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
-    r = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
-    t = (sums[0][2] + sums[1][2]) + (sums[2][2] + sums[3][2]);
+    c = r = t = 0.f;
+#pragma unroll
+    for (int i = 0; i < LP_JOIN_WAVES; ++i) { c += sums[i][0]; r += sums[i][1]; t += sums[i][2]; }
     // (a maximum that is not finite leaves no probabilities)
     const float log_s = fabsf(m) < INFINITY ? logf(c) + log1pf(r / c) : NAN;
     if (tid == 0) {
@@ -211,12 +219,12 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float
         __syncthreads();
         if (ranked) {
             constexpr int AT_ONCE = 4;                    // groups of a wave that are on their way together
-            for (int g0 = w; g0 < held; g0 += AT_ONCE * LP_WAVES) {
+            for (int g0 = w; g0 < held; g0 += AT_ONCE * LP_JOIN_WAVES) {
                 float v[AT_ONCE][4];
                 int from[AT_ONCE];
 #pragma unroll
                 for (int i = 0; i < AT_ONCE; ++i) {
-                    const int g = g0 + i * LP_WAVES;
+                    const int g = g0 + i * LP_JOIN_WAVES;
                     from[i] = g < held ? chosen[g] * LP_GROUP + 4 * lane : V;
                     load_four(src, from[i], V, v[i]);
                 }
@@ -284,7 +292,9 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_join_kernel(const float
 
 static int row_shares(int V, int u) { return (V + LP_GROUP * u - 1) / (LP_GROUP * u); }
 static int groups_of(int V) { return (V + LP_GROUP - 1) / LP_GROUP; }
-static int share_groups(int n) { return n <= 16 ? 2 : 8; }
+// Groups of a wave: few where there are few rows, for more waves.  Two and eight, us with 20 alternatives: one row 11.3 and 12.1, 64 rows 21.1 and
+// 23.6, 128 rows 26.7 and 31.9, 512 rows 73.3 and 70.2.
+static int share_groups(int n) { return n <= 128 ? 2 : 8; }
 
 // Floats of workspace that li_token_logprobs takes for n rows of V logits.
 extern "C" long li_token_logprobs_work_floats(int n, int V) {
@@ -312,6 +322,6 @@ extern "C" int li_token_logprobs(const float* logits, long stride, const int* id
         if (u == 2) logprob_rows_kernel<2><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
         else logprob_rows_kernel<8><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
     }
-    logprob_join_kernel<<<n, 64 * LP_WAVES, top ? 4 * (groups + (top < groups ? top : groups) * LP_GROUP) : 0, stream>>>(logits, stride, V, shares, share, tops, groups, ids, logprob, entropy, top, top_ids, top_logprob);
+    logprob_join_kernel<<<n, 64 * LP_JOIN_WAVES, top ? 4 * (groups + (top < groups ? top : groups) * LP_GROUP) : 0, stream>>>(logits, stride, V, shares, share, tops, groups, ids, logprob, entropy, top, top_ids, top_logprob);
     return li_launch_status();
 }
