@@ -721,7 +721,7 @@ struct MassPlan {
     long stride = 0;                     // keys of a head's scores
     int parts = 0, block_lds = 0;
     bool one_block = false;              // short contexts of single tokens: one kernel
-    int row_splits = 1, key_splits = 1, row_st = 1, row_share = 1, key_share = 1, stage = 64;      // (shares: stages, pairs)
+    int row_splits = 1, key_splits = 1, row_st = 1, key_st = 1, row_share = 1, key_share = 1, stage = 64;      // (shares: stages, pairs)
     long places = 0;                     // of the longer segments' sums, all together
     long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
     bool tiled = false, valid = false;
@@ -735,10 +735,12 @@ static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, cons
     return tokens * (q_row_stride * (long)es / 16) < 1L << 32 && rows * (dh * es / 16) < 1L << 32 && tokens * nh < 1L << 31 && dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
 }
 
+// Places of a segment's sums: whole blocks of keys.
+static long places_of(int ctx) { return (ctx + 64 * PT_WAVES - 1) / (64 * PT_WAVES) * (64L * PT_WAVES); }
+
 static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, bool f32, bool tiled) {
     MassPlan p;
     long total = 0;
-    const int keys = 32 * PT_WAVES * (f32 ? 1 : 2);
     for (int i = 0; i < nseg; ++i) {
         const int ctx = padded_ctx > 0 ? padded_ctx : ctx_len[i];
         if (q_len[i] <= 0 || ctx < q_len[i]) return p;
@@ -750,7 +752,7 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
             ++p.multi;
             p.multi_ctx = ctx > p.multi_ctx ? ctx : p.multi_ctx;
             p.multi_q = q_len[i] > p.multi_q ? q_len[i] : p.multi_q;
-            p.places += (ctx + keys - 1) / keys * (long)keys;
+            p.places += places_of(ctx);
         }
     }
     if (total != tokens || p.places >= 1L << 31) return p;
@@ -773,31 +775,41 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
     }
     if (p.multi) {
         // Blocks of about equal length: as many as the compute units hold at a time, each with no less than 8 stages of keys (4 pairs of a head and a stage
-        // of queries), or, where there is work for many rounds, 96 stages (40 pairs) each.  Rows: a wave holds two tiles of queries where that
-        // leaves a whole round of such blocks.  A prompt of 2,048 of 28 heads on 4, us with least 4, 8, 12 and 16 pairs: 83, 88, 87, 81; 990 tokens of 12
-        // heads on 2 behind 500: 37, 40, 48, 51; 512 of 28 heads behind 4,000: 60, 65, 69, 74; 1,999 of 40 heads behind 16,000: 750 with all.
+        // of queries), or, where there is work for many rounds, 96 stages (40 or 80 pairs) each.  A wave holds two tiles where that leaves blocks of
+        // some length, else one, and there are more of them.  Rows: two from 16 stages a block on.  Keys: two from 20 pairs a block on; one and two, us of both
+        // passes: a prompt of 2,048 of 28 heads on 4 79 and 87, of 512 of 14 heads on 2 21 and 26, 990 of 12 heads on 2 behind 500 33 and 36, 4 x 512 of 28
+        // heads behind 1,000 68 and 78 (8 to 14 pairs); 2,048 behind 2,000 149 and 149 (21); a prompt of 4,000 of 28 heads 195 and 191 (28), 2,048 behind
+        // 8,000 375 and 334, 1,999 of 40 heads on 8 behind 16,000 850 and 788 (166).
         const int rows = 32 * stage_tiles((dh <= 64 ? 64 : dh <= 128 ? 128 : 256) * (f32 ? 4 : 2));
         for (p.row_st = f32 ? 1 : 2;; p.row_st = 1) {
-            long stages = 0, most = 0;
+            long stages = 0, most = 0, all = 0;
             for (int i = 0; i < nseg; ++i) {
                 if (q_len[i] < 2) continue;
                 const long tiles = (q_len[i] + 32 * p.row_st - 1) / (32 * p.row_st), blocks = (tiles * rep + PT_WAVES - 1) / PT_WAVES;
+                all += blocks * nkv;
                 stages += blocks * nkv * ((ctx_len[i] - q_len[i] / 2 + rows - 1) / rows);
                 most = std::max(most, (long)(ctx_len[i] + rows - 1) / rows);
             }
             const long one = p.row_st == 2 || f32 ? 512 : 768;
-            p.row_share = (int)std::min(std::max((stages + one - 1) / one, 8L), 96L);
+            // (a block's last share is half a share on average)
+            const long fit = 2 * one > all ? (2 * stages + 2 * one - all - 1) / (2 * one - all) : 96;
+            p.row_share = (int)std::min(std::max(fit, 8L), 96L);
             p.row_share = (int)std::max((long)p.row_share, (most + 511) / 512);
             p.row_splits = (int)((most + p.row_share - 1) / p.row_share);
             if (p.row_st == 1 || stages >= one * 16) break;
         }
-        long units = 0;
-        for (int i = 0; i < nseg; ++i) {
-            if (q_len[i] < 2) continue;
-            const long n = (q_len[i] + rows - 1) / rows, base = ctx_len[i] - q_len[i];
-            units += (long)nkv * rep * (base / keys * n + ((ctx_len[i] + keys - 1) / keys - base / keys) * (n + 1) / 2);
+        for (p.key_st = f32 ? 1 : 2;; p.key_st = 1) {
+            const int keys = 32 * PT_WAVES * p.key_st;
+            const long one = p.key_st == 2 || f32 ? 512 : 768;
+            long units = 0;
+            for (int i = 0; i < nseg; ++i) {
+                if (q_len[i] < 2) continue;
+                const long n = (q_len[i] + rows - 1) / rows, base = ctx_len[i] - q_len[i];
+                units += (long)nkv * rep * (base / keys * n + ((ctx_len[i] + keys - 1) / keys - base / keys) * (n + 1) / 2);
+            }
+            p.key_share = (int)std::min(std::max((units + one - 1) / one, 4L), p.key_st == 2 || f32 ? 40L : 80L);
+            if (p.key_st == 1 || units >= one * 20) break;
         }
-        p.key_share = (int)std::min(std::max((units + 511) / 512, 4L), 40L);
         const long longest = (long)rep * ((p.multi_q + rows - 1) / rows);
         p.key_share = (int)std::max((long)p.key_share, (longest + 32767) / 32768);
         p.key_splits = (int)((longest + p.key_share - 1) / p.key_share);
@@ -827,7 +839,7 @@ static bool allow_lds(K kernel, int bytes) {
 template <typename T, int DHP>
 static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, bool padded,
                              int nseg, int tokens, float* work, hipStream_t stream) {
-    constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1, KEYS = 32 * ST * PT_WAVES;
+    constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1;
     constexpr int LDS_BYTES = PT_BUFS * 32 * stage_tiles(DHP * (int)sizeof(T)) * DHP * (int)sizeof(T);
     if (p.single) {
         for (int at = 0, i = 0; at < p.single;) {
@@ -859,7 +871,8 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
     }
     if (p.multi) {
         const auto rows = p.row_st == ST ? mass_rows_tile_kernel<T, DHP, ST> : mass_rows_tile_kernel<T, DHP, 1>;
-        const auto keys = mass_keys_tile_kernel<T, DHP, ST>;
+        const auto keys = p.key_st == ST ? mass_keys_tile_kernel<T, DHP, ST> : mass_keys_tile_kernel<T, DHP, 1>;
+        const int keys_block = 32 * PT_WAVES * p.key_st;
         if (!allow_lds(rows, LDS_BYTES) || !allow_lds(keys, LDS_BYTES)) return LI_ERR_LAUNCH;
         const int rep = a.nh / a.nkv, tiles = (p.multi_q + 32 * p.row_st - 1) / (32 * p.row_st);
         float2* stats = (float2*)(work + p.rows);
@@ -873,7 +886,7 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                 for (; i < nseg && n < EV_LIST; ++i)
                     if (b.q_len[i] > 1) {
                         list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = b.q_len[i]; list.ctx[n] = b.ctx_len[i]; list.off[n++] = (int)off;
-                        off += (b.ctx_len[i] + KEYS - 1) / KEYS * (long)KEYS;
+                        off += places_of(b.ctx_len[i]);
                     }
                 list.n = n;
                 at += n;
@@ -881,9 +894,9 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                     rows<<<dim3((tiles * rep + PT_WAVES - 1) / PT_WAVES * a.nkv, 1, n * p.row_splits), 64 * PT_WAVES, LDS_BYTES, stream>>>(
                         q, k, a, list, stats, lse, p.row_splits, p.row_share, tokens);
                 } else {
-                    keys<<<dim3((p.multi_ctx + KEYS - 1) / KEYS * a.nkv, p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
+                    keys<<<dim3((p.multi_ctx + keys_block - 1) / keys_block * a.nkv, p.key_splits, n), 64 * PT_WAVES, LDS_BYTES, stream>>>(
                         q, k, a, list, lse, sums, p.key_share, tokens, p.places);
-                    mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, KEYS, p.stage, p.key_share, p.places, mass);
+                    mass_join_kernel<<<dim3((p.multi_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, sums, keys_block, p.stage, p.key_share, p.places, mass);
                 }
             }
             if (pass == 0 && p.row_splits > 1) mass_lse_kernel<<<(unsigned)((rows_n + 255) / 256), 256, 0, stream>>>(stats, p.row_splits, rows_n, lse);
@@ -1194,8 +1207,11 @@ extern "C" int li_evict_select(const float* mass, const int* block_table, int ma
                           page_size % 4 == 0 && (uintptr_t)mass % 16 == 0};
     const long room = (long)max_blocks * page_size;      // (as long as any request can be; the tables say no more)
     const dim3 grid(nkv, n, entries);
+    // (More threads with fewer places each until their barriers cost more; us: 8 requests of 4,000 x 28 entries x 4 heads with 256, 512 and 1,024 threads
+    // 18.8, 16.5 and 24.5, of 1,000 8.3, 13.8 and 20.8; of 16,000 with 512 and 1,024 63 and 79, but 19.0 and 17.3 where each has a compute unit to itself.)
     if (room <= 1024) evict_select_kernel<256, 4><<<grid, 256, 0, stream>>>(a);
-    else if (room <= 4096) evict_select_kernel<256, 16><<<grid, 256, 0, stream>>>(a);
+    else if (room <= 4096) evict_select_kernel<512, 8><<<grid, 512, 0, stream>>>(a);
+    else if (room <= 16384 && (long)entries * n * nkv > 256) evict_select_kernel<512, 32><<<grid, 512, 0, stream>>>(a);
     else if (room <= 16384) evict_select_kernel<1024, 16><<<grid, 1024, 0, stream>>>(a);
     else if (room <= 32768) evict_select_kernel<1024, 32><<<grid, 1024, 0, stream>>>(a);
     else evict_select_long_kernel<<<grid, SEL_NT, 0, stream>>>(a);

@@ -69,6 +69,12 @@ def test_mass_of_a_long_portion_and_long_contexts(dtype):
     check_mass([(700, 700), (1, 2049), (300, 900)], 14, 2, 64, 16, dtype, ws=Workspace(DEV))
 
 
+@pytest.mark.parametrize("nh,nkv,dh,ctx,holes", [(64, 2, 64, 3410, []), (64, 8, 80, 3411, [(0, 3), (0, 40), (0, 213)]), (32, 2, 128, 6333, []), (17, 1, 256, 10800, [(0, 0)])])
+def test_mass_of_portions_with_work_for_many_rounds(nh, nkv, dh, ctx, holes):
+    """So many pairs of a head and a stage of queries that a wave takes two tiles of keys."""
+    check_mass([(910, ctx), (1, 33), (70, 75)], nh, nkv, dh, 16, torch.bfloat16, holes=holes)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_mass_that_adds_to_keys_of_another_entry(dtype):
     check_mass([(1, 70), (40, 90), (2, 2)], 12, 2, 128, 16, dtype, fresh=False)
