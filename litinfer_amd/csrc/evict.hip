@@ -59,7 +59,8 @@ __device__ __forceinline__ long some_row(const MassArgs& a, const int* table, in
     return r < 0 ? (long)kvh * a.page_size : r;
 }
 
-// ---- any head size, type and alignment: scores by the vector ALU, computed twice
+// ---- any head size, type and alignment: scores by the vector ALU, computed twice.  Nothing here is made for speed: rows of whole 16 bytes on 16 bytes, which
+// models have, go the other ways.
 template <typename T>
 __device__ __forceinline__ float dot_rows(const float* q, const T* k, int dh) {
     float s = 0.f;
@@ -154,7 +155,9 @@ __device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x
 }
 
 // ---- single tokens.  The scores themselves are kept (4 bytes a query head and key beside the key's dh * 2): reading the keys
-// again would cost more.
+// again would cost more.  Bound by the keys' way from memory and, at these sizes, by the launches around it: 64 requests of 100 to 2,001 keys, 12 heads on 2 of 128
+// bfloat16 (36 MB), 13.8 us for the scores and 5.3 for the sums; 3 of 20,000 to 32,001 keys, 28 heads on 4 of 128 float32 (162 MB), 39.6 (4.0 TB/s) and 12.1; one
+// of 300 keys, 14 heads on 2, 6.2 in one kernel.
 #define SG_KEYS 64                // keys of a wave
 #define SG_WAVES 4
 
@@ -317,8 +320,10 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
 // in different banks.
 //
 // A step is one tile of 32 staged rows: its products, beside them the exponentials of the tile before (MFMAs and the vector ALU work side by
-// side), and the first pieces of the next tile's rows, which then wait in registers.  What bounds a step is the exponentials and sums:
-// 96 vector instructions against 16 MFMAs.
+// side), and the first pieces of the next tile's rows, which then wait in registers.  What bounds a step is both together: of two tiles of bfloat16 rows of 128, 16
+// MFMAs alone take 262 ns, the 32 exponentials 120, the 64 other vector instructions 115, interleaved 329.  1,999 queries of 40 heads on 8 behind 16,000
+// keys: rows' statistics 425 to 450 us, columns' sums 378 to 400 (870 to 920 TFLOP/s of products each; the log of a row's sum is wanted before
+// the first weight can be added, so that all products are made twice).
 #define PT_WAVES 4
 #define PT_BUFS 3
 #define PT_RING 4                 // pieces of a row that are read ahead
@@ -396,8 +401,9 @@ __device__ __forceinline__ void in_steps(int n, Step step) {
 }
 
 // The rows' statistics: a wave holds ST * 32 queries of one head, the block streams keys.  Wave tiles of a kv head are numbered from the
-// last queries, whose rows are the longest, to the first, a tile's heads side by side: the four that a block takes see about the same keys.  grid: x kv heads times wave tiles / 4 (of the longest segment), z segments * splits; a split is `share` stages of keys.  The kv head
-// goes fastest, here and below: blocks go round the XCDs, so an XCD's second-level cache holds one kv head's rows, or a few.
+// last queries, whose rows are the longest, to the first, a tile's heads side by side: the four that a block takes see about the same keys.
+// grid: x kv heads times wave tiles / 4 (of the longest segment), z segments * splits; a split is `share` stages of keys.  The kv head goes fastest,
+// here and below: blocks go round the XCDs, so an XCD's second-level cache holds one kv head's rows, or a few.
 // stats [splits, nh, T], or, where there is one split, lse [nh, T] itself.
 template <typename T, int DHP, int ST>
 __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
@@ -1004,6 +1010,8 @@ __device__ __forceinline__ int block_before(int v, int* smem, int& all) {
 // digit: 256 equal parts of the range between the contest's least and its largest are counted in LDS, then those of the part in which the least
 // taken sum lies, and so on, until all of a part is taken or it is a single value, of whose places the lowest are taken.  (Equal parts of
 // the floats' order, not their leading bits: sums lie within a few octaves, and would meet in a few counters.)
+// Bound by that chain, two trips to memory and eight to twelve barriers, not by the 4 bytes a place: 8 requests of 2,500 to 4,096 places x 28 entries x 4 kv heads (19 MB)
+// 16.2 us, 8 entries x 8 kv heads of 32,000 (9 MB) 26.6.  (Halving by ballots of a bit a time took 35 and 56.)
 template <int NT, int VPT>
 __global__ __launch_bounds__(NT) void evict_select_kernel(SelectArgs a) {
     constexpr int W = NT / 64;
@@ -1243,6 +1251,8 @@ struct CompactTensors {
 // kept is ascending, so kept[j] >= j: rows that are read lie at or behind those that are written, and rows of a later chunk behind
 // all that an earlier one writes.  So a chunk's rows may be asked for any time before, and have to have arrived, for all threads, before it is
 // written: the chunk behind is on its way while one waits at the barrier and is written.  Where a row stays, or has no page, nothing is written.
+// Bound by memory: 8 requests of 2,500 to 4,096 cut to 2,048, 28 entries, 4 kv heads, keys and values of 128 bfloat16 and the sums (1.9 GB read and written) 394 to 431 us,
+// 4.4 to 4.8 TB/s where a large copy gets 4.7.
 template <typename V>
 __device__ __forceinline__ void compact_rows(V* __restrict__ data, int pieces, uint32_t inv, const int* __restrict__ kept, int K, const int* __restrict__ table,
                                              int max_blocks, int kvh, int nkv, int page_size, uint32_t page_inv, int num_pages,
