@@ -53,6 +53,8 @@ __device__ __forceinline__ long place_row(const MassArgs& a, const int* table, i
     if (page < 0 || page >= a.num_pages) return -1;
     return ((long)page * a.nkv + kvh) * a.page_size + rest;
 }
+// A segment's length on the device, no more than there is room for in the table and where `most` places were laid out (a replay may be told anything).
+__device__ __forceinline__ int device_ctx(const MassArgs& a, int seg, int most) { return min(min(a.ctx_len[seg], most), a.max_blocks * a.page_size); }
 // the row of a place, some row where there is none (whoever asks does not use it)
 __device__ __forceinline__ long some_row(const MassArgs& a, const int* table, int kvh, int t) {
     const long r = place_row(a, table, kvh, t);
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(64) void mass_rows_kernel(const T* __restrict__ q, 
     __shared__ float qs[EV_MAX_DH];
     const int seg = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x;
     if (i >= a.q_len[seg]) return;
-    const int tok = a.q_start[seg] + i, seen = min(a.ctx_len[seg], a.max_blocks * a.page_size) - a.q_len[seg] + i + 1;
+    const int tok = a.q_start[seg] + i, seen = device_ctx(a, seg, 0x7fffffff) - a.q_len[seg] + i + 1;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
     for (int d = lane; d < a.dh; d += 64) qs[d] = load_as_float(q + (size_t)tok * a.q_row_stride + (size_t)h * a.dh + d);
     __syncthreads();
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void mass_keys_kernel(const T* __restrict__ q,
                                                         float* __restrict__ mass) {
     __shared__ float qs[4][EV_MAX_DH], part[4][64];
     const int seg = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int nq = a.q_len[seg], ctx = min(a.ctx_len[seg], a.max_blocks * a.page_size), t = blockIdx.x * 64 + lane, rep = a.nh / a.nkv;
+    const int nq = a.q_len[seg], ctx = device_ctx(a, seg, 0x7fffffff), t = blockIdx.x * 64 + lane, rep = a.nh / a.nkv;
     if ((int)blockIdx.x * 64 >= ctx) return;
     const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
     const int base = ctx - nq;                           // place of the step's first token
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const
                                                                            float* __restrict__ scores, long stride, float2* __restrict__ stats, int parts) {
     const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, rep = a.nh / a.nkv;
     const int k0 = (blockIdx.x * SG_WAVES + (threadIdx.x >> 6)) * SG_KEYS;
-    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS);
+    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, parts * SG_KEYS);
     if (k0 >= ctx) return;
     const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
     const size_t head0 = (size_t)req * a.nh + (size_t)kvh * rep;
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * block_waves(CH)) void mass_single_block_kernel
     constexpr int WAVES = block_waves(CH);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int req = blockIdx.y, seg = list.n ? list.seg[req] : req, kvh = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, rep = a.nh / a.nkv;
-    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], stride), parts = stride / SG_KEYS;
+    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, stride), parts = stride / SG_KEYS;
     float* scores = reinterpret_cast<float*>(lds);
     float2* stats = reinterpret_cast<float2*>(scores + (size_t)rep * stride);
     float* lse = reinterpret_cast<float*>(stats + rep * parts);
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
                                                               const float2* __restrict__ stats, int parts, float* __restrict__ mass) {
     __shared__ float lse[SG_LSE];
     const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int ctx = list.n ? list.ctx[req] : min(a.ctx_len[seg], parts * SG_KEYS), t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
+    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, parts * SG_KEYS), t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
     if ((int)blockIdx.x * 256 >= ctx) return;
     const int n = (ctx + SG_KEYS - 1) / SG_KEYS;
     const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list
 // ---- the plan of a batch, from its segments in host memory: which kernels, how many splits, where things lie in the workspace
 struct MassPlan {
     int single = 0, multi = 0;           // segments of one token, of more
-    int single_ctx = 0, multi_ctx = 0, multi_q = 0;
+    int device_ctx = 0, multi_ctx = 0, multi_q = 0;
     long stride = 0;                     // keys of a head's scores
     int parts = 0, block_lds = 0;
     bool one_block = false;              // short contexts of single tokens: one kernel
@@ -753,7 +755,7 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
         total += q_len[i];
         if (q_len[i] == 1 && tiled) {
             ++p.single;
-            p.single_ctx = ctx > p.single_ctx ? ctx : p.single_ctx;
+            p.device_ctx = ctx > p.device_ctx ? ctx : p.device_ctx;
         } else {
             ++p.multi;
             p.multi_ctx = ctx > p.multi_ctx ? ctx : p.multi_ctx;
@@ -767,13 +769,13 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
     const int rep = nh / nkv;
     if (!tiled) { p.floats = (long)tokens * nh; return p; }
     if (p.single) {
-        p.parts = (p.single_ctx + SG_KEYS - 1) / SG_KEYS;
+        p.parts = (p.device_ctx + SG_KEYS - 1) / SG_KEYS;
         p.stride = (long)p.parts * SG_KEYS;
         const long lds = 4 * (rep * p.stride + 2L * rep * p.parts + rep);
         // One kernel where a block has few keys, or where the blocks fill the compute units, us: bfloat16, 28 heads on 4 of 128, one request of 300 keys 9.0
         // (two kernels) and 6.8, 64 requests 13.3 and 7.1, of 1,000 20.0 and 14.8, of 2,000 32.5 and 25.6; 8 requests of 1,000 9.4 and 12.8, 64
         // of 2,000 on 2 kv heads 20.3 and 23.5.
-        p.one_block = lds <= 150 * 1024 && (p.single_ctx <= 512 || ((long)p.single * nkv >= 192 && p.single_ctx <= 2048));
+        p.one_block = lds <= 150 * 1024 && (p.device_ctx <= 512 || ((long)p.single * nkv >= 192 && p.device_ctx <= 2048));
         p.block_lds = (int)lds;
         p.scores = 0;
         p.stats = p.one_block ? 0 : (long)p.single * nh * p.stride;
@@ -871,7 +873,7 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
             float2* stats = (float2*)(work + p.stats) + (size_t)at * a.nh * p.parts;
             mass_single_scores_kernel<T, CH16><<<dim3((p.parts + SG_WAVES - 1) / SG_WAVES, a.nkv, n), 64 * SG_WAVES, 0, stream>>>(
                 q, k, a, list, scores, p.stride, stats, p.parts);
-            mass_single_add_kernel<<<dim3((p.single_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, scores, p.stride, stats, p.parts, mass);
+            mass_single_add_kernel<<<dim3((p.device_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, scores, p.stride, stats, p.parts, mass);
             at += n;
         }
     }

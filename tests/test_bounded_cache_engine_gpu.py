@@ -9,7 +9,7 @@ import helpers
 import plain_impl
 from litinfer_amd.engine import Engine, Scheduler, StepEntry
 from litinfer_amd.models import Qwen2
-from tiny_configs import TINY_A, TINY_C, TINY_D, TINY_E
+from tiny_configs import TINY_A, TINY_B, TINY_C, TINY_D, TINY_E
 
 pytestmark = pytest.mark.gpu
 
@@ -127,6 +127,18 @@ def test_score(tmp_path):
     assert max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4 and max(abs(r.entropy - a) for r, a in zip(rows, entropy)) < 1e-4
     top = torch.sort(y, dim=1, descending=True).values[:, :5].tolist()
     assert max(abs(v - e) for r, t in zip(rows, top) for (_, v), e in zip(r.top, t)) < 1e-4
+
+
+@pytest.mark.parametrize("chunk", [64, 7])
+def test_score_with_windowed_layers(tmp_path, chunk):
+    d = helpers.make_model(tmp_path, TINY_B, 3)
+    raw, w = plain_impl.load_folder(d)
+    m = Qwen2(d, dtype="float32", page_size=8, max_tokens=1024, max_seqs=2, chunk_size=chunk)
+    toks = text(120, raw["vocab_size"])
+    y = torch.log_softmax(torch.from_numpy(plain_impl.forward(raw, w, toks)), 1)[:-1]
+    rows = m.score(toks)
+    want = y.gather(1, torch.tensor(toks[1:])[:, None])[:, 0].tolist()
+    assert len(rows) == 119 and max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4
 
 
 def test_two_engines_take_turns(tmp_path):

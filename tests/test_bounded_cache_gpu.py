@@ -211,6 +211,41 @@ def test_mass_in_a_recording_and_on_another_stream():
     assert torch.allclose(mass.cpu().double(), plain, rtol=mass_tolerance(qkv, k, meta, 12, 2, 128, 128 ** -0.5), atol=1e-30)
 
 
+@pytest.mark.parametrize("segs", [[(1, 30), (1, 31)], [(1, 700), (1, 90)]])
+def test_mass_of_a_replay_that_is_told_more_than_the_tables_hold(segs):
+    """Lengths are cut to the tables: nothing behind them is read or written."""
+    qkv, mass, k, meta = mass_inputs(segs, 4, 2, 64, 5, torch.bfloat16)
+    meta.padded = True
+    args = (4, 2, 64, 5, 0.125)
+    room = meta.max_blocks * 5
+    start = mass.clone()
+    meta.ctx_len.fill_(room)
+    ops.attention_mass(qkv, mass, k, meta, *args)
+    want = mass.clone()
+    mass.copy_(start)
+    meta.ctx_len.fill_(room + 1000)
+    ops.attention_mass(qkv, mass, k, meta, *args)
+    assert torch.equal(mass, want) and torch.isfinite(mass).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mass_of_portions_in_a_recording(dtype):
+    qkv, mass, k, meta = mass_inputs([(1, 130), (97, 260), (1, 33), (300, 300)], 12, 2, 128, 16, dtype)
+    args = (k, meta, 12, 2, 128, 16, 128 ** -0.5)
+    start, ws = mass.clone(), Workspace(DEV)
+    ops.attention_mass(qkv, mass, *args, ws=ws)
+    want = mass.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_mass(qkv, mass, *args, ws=ws)
+    for _ in range(3):
+        mass.copy_(start)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mass, want)
+        torch.randn(100000, device=DEV).sum().item()
+
+
 # ------------------------------------------------------------------------------------- evict_select, cache_compact
 def cache(lens, entries, nkv, page_size, seed=0, holes=()):
     meta, pages = cases.batch([(1, max(n, 1)) for n in lens], page_size, DEV, seed, holes=holes)
