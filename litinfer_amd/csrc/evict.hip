@@ -335,6 +335,10 @@ constexpr int stage_tiles(int row_bytes) { return PT_BUFS * 64 * row_bytes <= 15
 __device__ __forceinline__ void load_to_lds(const void* src, uint32_t at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(src) : "memory", "m0");
 }
+// The same from `base`, the same in all lanes, and `offset` bytes.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(base) : "memory", "m0");
+}
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 
 // The wave's loads but the `LATER` youngest have arrived, and with them, behind the barrier, all waves' (a wave's loads retire in order).
@@ -346,15 +350,14 @@ __device__ __forceinline__ void arrived() {
 template <int PPR>
 __device__ __forceinline__ int swizzle(int r) { return r & (PPR < 16 ? PPR - 1 : 15); }
 
-// All waves: ROWS rows, row r from the piece row_at(r) of src on, `pieces` of 16 bytes a row, PPR places a row.
-template <int PPR, int ROWS, typename RowAt>
-__device__ __forceinline__ void stage_rows(char* lds, const void* src, int pieces, int w, int lane, RowAt row_at) {
+// All waves bring ROWS rows, PPR places a row: load(i, row, piece, offset in LDS of the lanes' first place) for a lane's i-th place.
+template <int PPR, int ROWS, typename Load>
+__device__ __forceinline__ void stage_rows(uint32_t at, int w, int lane, Load load) {
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int first = (w * LOADS + i) * 64, slot = first + lane, r = slot / PPR, p = (slot % PPR) ^ swizzle<PPR>(r);
-        const uint32_t piece = row_at(r) + p;
-        if (p < pieces) load_to_lds((const u32x4_t*)src + piece, lds_offset(lds) + 16 * first);
+        const int first = (w * LOADS + i) * 64, slot = first + lane, r = slot / PPR;
+        load(i, r, (slot % PPR) ^ swizzle<PPR>(r), at + 16 * first);
     }
 }
 // Where a lane's pieces of its row lie in a tile.
@@ -450,6 +453,7 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     for (int x = 0; x < ST; ++x) { m[x] = -INFINITY; l[x] = 0.f; }
     // (the rows of a stage are looked up in the table a stage before they are asked for, one a lane)
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
+    const uint32_t lds0 = lds_offset(lds);
     uint32_t row = 0;                                    // in pieces
     uint64_t next_there = 0, there[PT_BUFS];             // which of a stage's keys have a page
     auto look_up = [&](int s) __attribute__((always_inline)) {
@@ -460,7 +464,15 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     auto load = [&](auto which_buf) __attribute__((always_inline)) {
         constexpr int buf = decltype(which_buf)::value;
         there[buf] = next_there;
-        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, k, pieces, w, lane, [&](int r) { return (uint32_t)__shfl((int)row, r, LI_WAVE); });
+        if (pieces == PPR)                               // (whole rows need no mask, whose branches cost more than the loads)
+            stage_rows<PPR, ROWS>(lds0 + buf * STAGE_BYTES, w, lane, [&](int, int r, int p, uint32_t to) __attribute__((always_inline)) {
+                load_to_lds((const u32x4_t*)k + ((uint32_t)__shfl((int)row, r, LI_WAVE) + p), to);
+            });
+        else
+            stage_rows<PPR, ROWS>(lds0 + buf * STAGE_BYTES, w, lane, [&](int, int r, int p, uint32_t to) __attribute__((always_inline)) {
+                const uint32_t piece = (uint32_t)__shfl((int)row, r, LI_WAVE) + p;
+                if (p < pieces) load_to_lds((const u32x4_t*)k + piece, to);
+            });
     };
     int at[CH];
     staged_at<PPR>(c, half, at);
@@ -610,21 +622,29 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* 
     const int first = pairs.first, n = pairs.n;
     const int u0 = (int)((long)rep * n * split / pairs.splits), u1 = (int)((long)rep * n * (split + 1) / pairs.splits);
     int lh = u0 / n, ls = first + u0 % n;                // the pair that is loaded next
-    const uint32_t q_pieces = a.q_row_stride / PE;
+    const uint32_t lds0 = lds_offset(lds), q_bytes = (uint32_t)a.q_row_stride * sizeof(T);
+    uint32_t offset[LOADS];                              // of a lane's pieces from the stage's first row
+    stage_rows<PPR, ROWS>(0, w, lane, [&](int i, int r, int p, uint32_t) __attribute__((always_inline)) { offset[i] = r * q_bytes + 16 * p; });
     float lq[PT_BUFS][TPS];                              // the queries' lse of the stages on their way, and where these begin
     int from[PT_BUFS];
     auto load = [&](auto which_buf) __attribute__((always_inline)) {
         constexpr int buf = decltype(which_buf)::value;
         const int i0 = ls * ROWS;
+        const T* rows = q + (size_t)(tok0 + i0) * a.q_row_stride + (size_t)(kvh * rep + lh) * a.dh;
+        const float* row_lse = lse + (size_t)(kvh * rep + lh) * tokens + tok0 + i0;
         from[buf] = i0;
+        if (pieces == PPR && i0 + ROWS <= nq) {          // (whole rows, all of them there: no masks, whose branches cost more than the loads)
 #pragma unroll
-        for (int y = 0; y < TPS; ++y) {
-            const int i = i0 + 32 * y + c;
-            lq[buf][y] = i < nq ? lse[(kvh * rep + lh) * tokens + tok0 + i] : INFINITY;
+            for (int y = 0; y < TPS; ++y) lq[buf][y] = row_lse[32 * y + c];
+            stage_rows<PPR, ROWS>(lds0 + buf * STAGE_BYTES, w, lane,
+                                  [&](int i, int, int, uint32_t to) __attribute__((always_inline)) { load_to_lds(rows, offset[i], to); });
+        } else {
+#pragma unroll
+            for (int y = 0; y < TPS; ++y) lq[buf][y] = i0 + 32 * y + c < nq ? row_lse[32 * y + c] : INFINITY;
+            stage_rows<PPR, ROWS>(lds0 + buf * STAGE_BYTES, w, lane, [&](int, int r, int p, uint32_t to) __attribute__((always_inline)) {
+                if (p < pieces) load_to_lds(rows, min(r, nq - 1 - i0) * q_bytes + 16 * p, to);
+            });
         }
-        stage_rows<PPR, ROWS>(lds + buf * STAGE_BYTES, q, pieces, w, lane, [&](int r) {
-            return (uint32_t)(tok0 + min(i0 + r, nq - 1)) * q_pieces + (kvh * rep + lh) * pieces;
-        });
         if (++ls == first + n) { ls = first; ++lh; }
     };
     int at[CH];
@@ -737,10 +757,10 @@ struct MassPlan {
 
 struct Batch { const int *q_start, *q_len, *ctx_len; };      // in host memory
 
-// (the tiles' loads count pieces of 16 bytes in 32 bits)
+// (the tiles' loads count pieces of 16 bytes in 32 bits, and bytes of 64 rows)
 static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, const void* k, float scale, long tokens, long nh, long rows) {
     const int es = dtype == LI_BF16 ? 2 : 4;
-    return tokens * (q_row_stride * (long)es / 16) < 1L << 32 && rows * (dh * es / 16) < 1L << 32 && tokens * nh < 1L << 31 && dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
+    return tokens * (q_row_stride * (long)es / 16) < 1L << 32 && 64L * q_row_stride * es < 1L << 32 && rows * (dh * es / 16) < 1L << 32 && tokens * nh < 1L << 31 && dh * es % 16 == 0 && q_row_stride * (long)es % 16 == 0 && ((uintptr_t)q | (uintptr_t)k) % 16 == 0 && scale > 0.f && scale < INFINITY;
 }
 
 // Places of a segment's sums: whole blocks of keys.
