@@ -503,12 +503,12 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     // keys that a query does not see, if there may be any among these 32
     auto hide = [&](f32x16_t (&acc)[ST], int k0, uint32_t there) __attribute__((always_inline)) {
         if (there == ~0u && k0 + 31 <= seen_all) return;
-        there >>= 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int i = 8 * (r >> 2) + (r & 3);
+        for (int x = 0; x < ST; ++x) {
+            const int last_seen = pos[x] - k0;           // (a mask in bits: the compiler makes branches of two conditions)
+            const uint32_t seen = (there & (last_seen < 0 ? 0u : 0xffffffffu >> (31 - min(last_seen, 31)))) >> (4 * half);
 #pragma unroll
-            for (int x = 0; x < ST; ++x) acc[x][r] = (there >> i & 1) && k0 + 4 * half + i <= pos[x] ? acc[x][r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) acc[x][r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? acc[x][r] : -INFINITY;
         }
     };
     auto stay = [&]() __attribute__((always_inline)) {   // (the compiler would move the exponentials behind the branch that follows)
