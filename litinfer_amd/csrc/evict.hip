@@ -479,7 +479,7 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
     u32x4_t ring[PT_RING];
     // lane (c, half) gets query c's scores of keys 8 (r / 4) + 4 half + r % 4
     // A tile joins the rows' statistics in CH shares: the first quarter finds the maxima, the others add up.
-    float b[ST], sum[ST];
+    float b[ST], sum[ST][4];                             // (four sums: one would wait for itself)
     constexpr int LEAD = CH / 4, EACH = CH - LEAD;
     auto add_up = [&](const f32x16_t (&acc)[ST], int j) __attribute__((always_inline)) {
 #pragma unroll
@@ -492,12 +492,12 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
                 b[x] = fmaxf(mn, -1e30f);                // (nothing seen yet: 2^(-inf + 1e30) is nothing)
                 l[x] *= __builtin_amdgcn_exp2f(fmaxf(m[x], -1e30f) - b[x]);
                 m[x] = mn;
-                sum[x] = 0.f;
+                sum[x][0] = sum[x][1] = sum[x][2] = sum[x][3] = 0.f;
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (j >= LEAD && (16 * x + r) * EACH / (16 * ST) == j - LEAD) sum[x] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -b[x]));
-            if (j == CH - 1) l[x] += sum[x];
+                if (j >= LEAD && (16 * x + r) * EACH / (16 * ST) == j - LEAD) sum[x][r & 3] += __builtin_amdgcn_exp2f(fmaf(acc[x][r], a.scale, -b[x]));
+            if (j == CH - 1) l[x] += (sum[x][0] + sum[x][1]) + (sum[x][2] + sum[x][3]);
         }
     };
     // keys that a query does not see, if there may be any among these 32
@@ -589,7 +589,7 @@ __device__ __forceinline__ Pairs pairs_of(int b0, int base, int nq, int rep, int
 }
 
 template <typename T, int DHP, int ST>
-__global__ __launch_bounds__(64 * PT_WAVES) void mass_keys_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
+__global__ __launch_bounds__(64 * PT_WAVES, DHP * sizeof(T) <= 256 ? 2 : 1) void mass_keys_tile_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
                                                                        const float* __restrict__ lse, float* __restrict__ part, int share, int tokens, long places) {
     constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16, KEYS = 32 * ST;
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
