@@ -324,8 +324,8 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
 // A step is one tile of 32 staged rows: its products, beside them the exponentials of the tile before (MFMAs and the vector ALU work side by
 // side), and the first pieces of the next tile's rows, which then wait in registers.  What bounds a step is both together: of two tiles of bfloat16 rows of 128, 16
 // MFMAs alone take 262 ns, the 32 exponentials 120, the 64 other vector instructions 115, interleaved 329.  1,999 queries of 40 heads on 8 behind 16,000
-// keys: rows' statistics 425 to 450 us, columns' sums 378 to 400 (870 to 920 TFLOP/s of products each; the log of a row's sum is wanted before
-// the first weight can be added, so that all products are made twice).
+// keys: rows' statistics 417 to 448 us, columns' sums 354 to 374 (up to 830 and 980 TFLOP/s of products; matrix cores busy 38 and 47 %, the vector ALU 64 and 59; the log of a
+// row's sum is wanted before the first weight can be added, so that all products are made twice).
 #define PT_WAVES 4
 #define PT_BUFS 3
 #define PT_RING 4                 // pieces of a row that are read ahead
