@@ -387,6 +387,10 @@ class Scheduler:
                 break
         return plan
 
+    def largest_portion(self, rid: Hashable, n: int, cached: Optional[int] = None) -> int:
+        """The largest portion of at most `n` tokens whose pages are free now (0: not even one token's); cached: 0 for a request that is not live yet."""
+        return self._largest_fitting(self.cache.free_pages(), rid, n, cached)
+
     def keep_within_budget(self, rids: Sequence[Hashable]) -> None:
         """Cuts those of the live requests whose cache has outgrown the budget and its slack."""
         if self.cache_budget is None:

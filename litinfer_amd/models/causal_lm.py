@@ -129,7 +129,8 @@ class CausalLM:
 
     def score(self, inputs: Sequence[int], top: int = 0) -> List[TokenLogprob]:
         """What the model thinks of a given text: for every token behind the first, its log probability after those before it, the entropy there
-        and the `top` likeliest tokens.  With a `cache_budget` the text is read as a long prompt is, its cache cut between portions."""
+        and the `top` likeliest tokens.  The text is read in portions of at most `chunk_size` tokens, shorter where fewer pages are free; with
+        a `cache_budget` its cache is cut between them, as a long prompt's is."""
         tokens = self._check(inputs, 1, "score")
         top = check_top(top, self.engine.spec.vocab_size, "score")
         vocab = self.engine.spec.vocab_size
@@ -139,11 +140,15 @@ class CausalLM:
         pending, given = [], torch.tensor(tokens[1:], dtype=torch.int32).to(engine.rt.device)
         try:
             portion = min(sched.chunk_size, sched.max_batch_tokens)
-            for at in range(0, len(given), portion):
-                part = tokens[at:min(at + portion, len(given))]
+            at = 0
+            while at < len(given):
+                # (where not even one token fits, the step says what is missing)
+                n = sched.largest_portion(rid, min(portion, len(given) - at), None if at else 0)
+                part = tokens[at:at + max(n, 1)]
                 logits = engine.step([StepEntry(rid, part, range(len(part)))])
                 pending.append(sched.sampler.logprobs_async(logits, given[at:at + len(part)], top))
                 sched.keep_within_budget([rid])
+                at += len(part)
             return [row for p in pending for row in p.result()]
         finally:
             engine.finish(rid)

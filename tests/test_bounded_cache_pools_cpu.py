@@ -1,0 +1,104 @@
+"""Requests with a bounded cache, and texts that are scored, in pools that hold little more than they need (stand-ins for the kernels)."""
+import numpy as np
+import pytest
+import torch
+
+import bounded_cache_cases as cases
+import helpers
+import plain_impl
+from litinfer_amd.cache import CacheFull
+from litinfer_amd.engine import Engine, Scheduler
+from litinfer_amd.kernels import ops
+from litinfer_amd.models import Qwen2
+from tiny_configs import TINY_A, TINY_B
+
+CFG = {**TINY_A, "max_position_embeddings": 512}
+
+
+@pytest.fixture
+def bounded_ops(cpu_ops, monkeypatch):
+    for f in cases.STAND_INS:
+        monkeypatch.setattr(ops, f.__name__, f)
+
+
+@pytest.fixture
+def model(tmp_path):
+    return helpers.make_model(tmp_path, CFG, 3)
+
+
+def text(n, seed=0, vocab=CFG["vocab_size"]):
+    return np.random.default_rng(seed).integers(0, vocab, n).tolist()
+
+
+def steps_of(eng):
+    """The numbers of tokens of the steps that the engine takes from now on."""
+    sizes, step = [], eng.step
+    eng.step = lambda entries: sizes.append(sum(len(e.tokens) for e in entries)) or step(entries)
+    return sizes
+
+
+# -------------------------------------------------------------------------------------------------- score
+def check_scored_in(model, toks, rows, sizes, budget, slack):
+    """The rows are those of the text in portions of `sizes`, its cache cut to `budget` where it has outgrown the slack."""
+    cfg, w = plain_impl.load_folder(model)
+    ref, at, want = cases.PlainBounded(cfg, w), 0, []
+    for n in sizes:
+        y = torch.log_softmax(torch.from_numpy(ref.step(toks[at:at + n])), 1)
+        want += y.gather(1, torch.tensor(toks[at + 1:at + 1 + n])[:, None])[:, 0].tolist()
+        at += n
+        if ref.cached > budget + slack:
+            ref.evict(budget)
+    assert at == len(toks) - 1 and [r.token for r in rows] == toks[1:]
+    assert max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4
+
+
+@pytest.mark.parametrize("pages", [22, 24, 28, 40])
+def test_score_takes_portions_that_fit_the_pool(bounded_ops, model, pages):
+    """budget 40, slack 128, portions of 64: 22 pages of 8 hold budget and slack and a token, 29 a whole portion too."""
+    m = Qwen2(model, device="cpu", dtype="float32", page_size=8, num_pages=pages, max_seqs=2, chunk_size=64, cache_budget=40)
+    toks = text(400)
+    assert len(m.generate(toks, max_new_tokens=3)) == 3
+    sizes = steps_of(m.engine)
+    rows = m.score(toks)
+    check_scored_in(model, toks, rows, sizes, 40, 128)
+    assert max(sizes) == 64 and (min(sizes[:-1]) < 64) == (pages < 29)
+    assert m.engine.cache.live() == [] and m.engine.cache.free_pages() == [pages]
+
+
+def test_score_beside_requests_that_hold_pages(bounded_ops, model):
+    m = Qwen2(model, device="cpu", dtype="float32", page_size=8, num_pages=30, max_seqs=3, chunk_size=64, cache_budget=40)
+    m.engine_start()
+    rid = m.engine_add_request(text(60, 5), 6)
+    m.engine_step()
+    held = len(m.engine.cache.block_table(rid, 0))
+    sizes = steps_of(m.engine)
+    toks = text(300, 1)
+    check_scored_in(model, toks, m.score(toks), sizes, 40, 128)
+    assert held == 8 and min(sizes[:-1]) < 64
+    while m.engine_has_unfinished():
+        m.engine_step()
+    assert len(m.engine_get_output(rid)) == 6
+
+
+def test_score_of_a_text_that_does_not_fit_at_all(bounded_ops, model):
+    m = Qwen2(model, device="cpu", dtype="float32", page_size=8, num_pages=10, max_seqs=2, chunk_size=64)
+    with pytest.raises(CacheFull):
+        m.score(text(100))
+    assert m.engine.cache.live() == [] and m.engine.cache.free_pages() == [10]
+    assert len(m.score(text(81))) == 80
+
+
+def test_score_with_windowed_layers_in_a_pool_of_little_more_than_the_window(bounded_ops, tmp_path):
+    d = helpers.make_model(tmp_path, TINY_B, 3, name="windowed")
+    raw, w = plain_impl.load_folder(d)
+    toks = text(100, 2, raw["vocab_size"])
+    y = torch.log_softmax(torch.from_numpy(plain_impl.forward(raw, w, toks)), 1)[:-1]
+    want = y.gather(1, torch.tensor(toks[1:])[:, None])[:, 0].tolist()
+    whole = Qwen2(d, device="cpu", dtype="float32", page_size=8, max_tokens=256, max_seqs=2, chunk_size=64)
+    window = max(g.need.reach for g in whole.engine.cache.groups)
+    assert window > 0
+    pages = [13 if g.need.reach <= 0 else -(-window // 8) + 2 for g in whole.engine.cache.groups]
+    m = Qwen2(d, device="cpu", dtype="float32", page_size=8, num_pages=pages, max_seqs=2, chunk_size=64)
+    sizes = steps_of(m.engine)
+    rows = m.score(toks)
+    assert max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4 and max(sizes) < 64
