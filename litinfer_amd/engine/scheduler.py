@@ -246,13 +246,13 @@ class Scheduler:
         self.preemptions += 1
         self.waiting.appendleft(req)
 
-    def _at_a_time(self, need, portion: Optional[int] = None):
+    def _at_a_time(self, need, portion: Optional[int] = None, held=None):
         """`need` (pages per group, a list or an array [requests, groups]) counts every page that a
         request's further tokens fill.  A windowed group gives pages back as the window passes them:
         there a request holds at most the window's pages and those of the portion that a step brings
         (up to `chunk_size` tokens) at a time, and that is what has to be free for it; a pool smaller
         than that serves one request at a time, in shorter portions.  With a `cache_budget` the same holds of
-        the budget, its slack and a portion."""
+        the budget, its slack and a portion; `held` [requests, groups] pages that the requests have already are part of it."""
         P = self.cache.page_size
         portion = self.chunk_size if portion is None else portion
         caps = [min(-(-(g.need.reach - 1 + portion) // P) + 1 + -(-g.need.keep_first // P), g.pool.capacity)
@@ -265,7 +265,9 @@ class Scheduler:
             need = need.copy()
             for gi, c in enumerate(caps):
                 if c is not None:
-                    np.minimum(need[:, gi], c, out=need[:, gi])
+                    # (a windowed request's pages are given back and taken anew, so what it holds says little of what it will take)
+                    bounded = held is not None and self.cache.groups[gi].need.reach <= 0
+                    np.minimum(need[:, gi], np.maximum(c - held[:, gi], 0) if bounded else c, out=need[:, gi])
             return need
         return [n if c is None else min(n, c) for n, c in zip(need, caps)]
 
@@ -341,8 +343,10 @@ class Scheduler:
             if self.waiting and budget > 0 and slots > 0 and len(self.running) < self.max_running:
                 going = [r for r in self.running if left[id(r)] > 0]
                 if going:
+                    held = None if self.cache_budget is None else \
+                        np.array([[self.cache.table_len(r.rid, g) for g in range(len(self.cache.groups))] for r in going])
                     need = self._at_a_time(self.cache.pages_needed_many(
-                        self.cache.handles_of([r.rid for r in going]), np.asarray([left[id(r)] for r in going], dtype=np.int32)))
+                        self.cache.handles_of([r.rid for r in going]), np.asarray([left[id(r)] for r in going], dtype=np.int32)), held=held)
                     spare = [int(a - b) for a, b in zip(spare, need.sum(axis=0))]
             while self.waiting and budget > 0 and slots > 0 and len(self.running) < self.max_running:
                 r = self.waiting[0]

@@ -102,3 +102,41 @@ def test_score_with_windowed_layers_in_a_pool_of_little_more_than_the_window(bou
     sizes = steps_of(m.engine)
     rows = m.score(toks)
     assert max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4 and max(sizes) < 64
+
+
+# ---------------------------------------------------------------------------------------------- scheduler
+def engine(d, **kw):
+    return Engine.from_dir(d, **{**dict(dtype="float32", device="cpu", page_size=8, max_seqs=4, attention_mass=True, page_order_seed=1), **kw})
+
+
+def run_two(model, pages, steps_before):
+    """Two prompts of 200, the second some steps after the first: how many steps both were running, the most pages that were held."""
+    eng = engine(model, num_pages=pages)
+    sched = Scheduler(eng, chunk_size=16, max_batch_tokens=64, cache_budget=24, cache_slack=8)
+    sched.add_request(text(200), 4, rid="a")
+    for _ in range(steps_before):
+        sched.step()
+    sched.add_request(text(200, 1), 4, rid="b")
+    both = 0
+    while sched.has_unfinished():
+        sched.step()
+        eng.cache.check_invariants()
+        both += len(sched.running) == 2
+    assert sched.preemptions == 0 and [len(sched.output(r)) for r in "ab"] == [4, 4]
+    return both
+
+
+@pytest.mark.parametrize("steps_before", [1, 2, 3, 5])
+def test_a_second_long_prompt_runs_beside_the_first_in_a_pool_of_two_peaks(bounded_ops, model, steps_before):
+    """A request holds at most ceil((24 + 8 + 16) / 8) = 6 pages at a time: what the first holds already is part of its six."""
+    assert run_two(model, 12, steps_before) >= 13 - steps_before - 1
+    assert run_two(model, 11, steps_before) <= 5                  # one page less: the second waits for the end of the first prompt (its last portion, four tokens)
+
+
+def test_what_a_windowed_request_holds_does_not_count_against_what_it_takes(bounded_ops, tmp_path):
+    """Without a budget nothing has changed: the windowed group's cap is what has to be free."""
+    d = helpers.make_model(tmp_path, TINY_B, 3, name="windowed")
+    sched = Scheduler(Engine.from_dir(d, dtype="float32", device="cpu", page_size=8, max_seqs=2, max_tokens=256))
+    need = np.full((2, len(sched.cache.groups)), 1000, dtype=np.int32)
+    held = np.full_like(need, 3)
+    assert (sched._at_a_time(need) == sched._at_a_time(need, held=held)).all()
