@@ -132,7 +132,7 @@ class CausalLM:
         and the `top` likeliest tokens.  The text is read in portions of at most `chunk_size` tokens, shorter where fewer pages are free; with
         a `cache_budget` its cache is cut between them, as a long prompt's is."""
         tokens = self._check(inputs, 1, "score")
-        top = check_top(top, self.engine.spec.vocab_size, "score")
+        top = check_top(top, self.engine.spec.vocab_size, "score", optional=False)
         vocab = self.engine.spec.vocab_size
         if min(tokens) < 0 or max(tokens) >= vocab:
             raise ValueError(f"score: a token id is outside the vocabulary of {vocab}")

@@ -151,9 +151,9 @@ class TokenLogprob:
         return self if len(self.top) == top else replace(self, top=self.top[:top])
 
 
-def check_top(top, vocab: int, who: str) -> Optional[int]:
-    """The number of alternatives that a caller asks for, or None where it asks for no log probabilities."""
-    if top is None:
+def check_top(top, vocab: int, who: str, optional: bool = True) -> Optional[int]:
+    """The number of alternatives that a caller asks for, or None where it asks for no log probabilities (if these are `optional`)."""
+    if top is None and optional:
         return None
     if isinstance(top, bool) or not isinstance(top, (int, np.integer)) or not 0 <= top <= min(ops.LOGPROBS_MAX_TOP, vocab):
         raise ValueError(f"{who}: the number of alternatives must lie between 0 and {min(ops.LOGPROBS_MAX_TOP, vocab)}, found {top!r}")
@@ -318,7 +318,7 @@ class Sampler:
     def logprobs_async(self, logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> PendingLogprobs:
         """The log probability of token ids[i] (int32, on the device) in row i of logits [n, vocab], the row's entropy and its `top` likeliest
         tokens, copied to the host without waiting."""
-        n, top = logits.shape[0], check_top(top, logits.shape[1], "logprobs")
+        n, top = logits.shape[0], check_top(top, logits.shape[1], "logprobs", optional=False)
         words = torch.empty(n * (3 + 2 * top), dtype=torch.int32, device=logits.device)
         values = words.view(torch.float32)
         words[:n].copy_(ids)

@@ -10,6 +10,7 @@ from litinfer_amd.cache import CacheFull
 from litinfer_amd.engine import Engine, Scheduler
 from litinfer_amd.kernels import ops
 from litinfer_amd.models import Qwen2
+from litinfer_amd.sampling import Sampler
 from tiny_configs import TINY_A, TINY_B
 
 CFG = {**TINY_A, "max_position_embeddings": 512}
@@ -102,6 +103,15 @@ def test_score_with_windowed_layers_in_a_pool_of_little_more_than_the_window(bou
     sizes = steps_of(m.engine)
     rows = m.score(toks)
     assert max(abs(r.logprob - a) for r, a in zip(rows, want)) < 1e-4 and max(sizes) < 64
+
+
+@pytest.mark.parametrize("top", [None, -1, 33, True, 1.5])
+def test_score_refuses_numbers_of_alternatives(bounded_ops, model, top):
+    m = Qwen2(model, device="cpu", dtype="float32", page_size=8, num_pages=30, max_seqs=2)
+    with pytest.raises(ValueError, match="score: the number of alternatives"):
+        m.score(text(9), top=top)
+    with pytest.raises(ValueError, match="logprobs: the number of alternatives"):
+        Sampler("cpu").logprobs_async(torch.zeros(2, 99), torch.zeros(2, dtype=torch.int32), top)
 
 
 # ---------------------------------------------------------------------------------------------- scheduler
