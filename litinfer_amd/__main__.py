@@ -33,6 +33,11 @@ def _perplexity(logprob: float, tokens: int):
         return math.inf
 
 
+def _finite(x):
+    """The number, or None (JSON has neither infinities nor NaN)."""
+    return x if x is not None and math.isfinite(x) else None
+
+
 def _cmd_generate(a) -> int:
     from .models import load
     if getattr(a, "test", False):
@@ -79,8 +84,9 @@ def _generate(a, load) -> int:
     if a.cmd == "score":
         rows = model.score(ids, top=a.top)
         total = sum(r.logprob for r in rows)
-        print(json.dumps({"tokens": len(rows), "logprob": total, "perplexity": _perplexity(total, len(rows)),
-                          "rows": [{"token": r.token, "logprob": r.logprob, "entropy": r.entropy, "top": [list(t) for t in r.top]} for r in rows]}))
+        print(json.dumps({"tokens": len(rows), "logprob": _finite(total), "perplexity": _finite(_perplexity(total, len(rows))),
+                          "rows": [{"token": r.token, "logprob": _finite(r.logprob), "entropy": _finite(r.entropy),
+                                    "top": [[t, _finite(p)] for t, p in r.top]} for r in rows]}, allow_nan=False))
         return 0
     tokens, metrics = model.generate_profile(ids, max_new_tokens=a.max_steps, top_k=a.top_k,
                                              top_p=a.top_p, temperature=a.temperature)
@@ -127,7 +133,7 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="python -m litinfer_amd")
     sub = ap.add_subparsers(dest="cmd", required=True)
     g = sub.add_parser("generate", help="generate tokens from a prompt")
-    sc = sub.add_parser("score", help="log probabilities of a given text's tokens")
+    sc = sub.add_parser("score", help="log probabilities of a given text's tokens, as a line of JSON (null: not a finite number)")
     for q in (g, sc):
         q.add_argument("--model", default=None, type=str)
         q.add_argument("--random", default=None, type=str, metavar="CONFIG.json",

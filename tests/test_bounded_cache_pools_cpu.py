@@ -1,4 +1,7 @@
 """Requests with a bounded cache, and texts that are scored, in pools that hold little more than they need (stand-ins for the kernels)."""
+import json
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -10,7 +13,7 @@ from litinfer_amd.cache import CacheFull
 from litinfer_amd.engine import Engine, Scheduler
 from litinfer_amd.kernels import ops
 from litinfer_amd.models import Qwen2
-from litinfer_amd.sampling import Sampler
+from litinfer_amd.sampling import Sampler, TokenLogprob
 from tiny_configs import TINY_A, TINY_B
 
 CFG = {**TINY_A, "max_position_embeddings": 512}
@@ -112,6 +115,21 @@ def test_score_refuses_numbers_of_alternatives(bounded_ops, model, top):
         m.score(text(9), top=top)
     with pytest.raises(ValueError, match="logprobs: the number of alternatives"):
         Sampler("cpu").logprobs_async(torch.zeros(2, 99), torch.zeros(2, dtype=torch.int32), top)
+
+
+def test_what_score_prints_is_json_whatever_the_numbers_are(bounded_ops, model, monkeypatch, capsys):
+    def score(self, ids, top=0):
+        return [TokenLogprob(7, -math.inf, 0.5, ((3, -0.25), (4, -math.inf))), TokenLogprob(8, math.nan, math.nan, ((3, math.nan), (4, math.nan))), TokenLogprob(9, -1e5, 1.0, ())]
+    monkeypatch.setattr(Qwen2, "score", score)
+    from litinfer_amd.__main__ import main
+    assert main(["score", "--model", str(model), "--device", "cpu", "--dtype", "float32", "--num-pages", "20", "--prompt-ids", "1,2,3,4"]) == 0
+
+    def refuse(name):
+        raise AssertionError(name)
+    out = json.loads(capsys.readouterr().out.splitlines()[-1], parse_constant=refuse)
+    assert out["logprob"] is None and out["perplexity"] is None
+    assert [r["logprob"] for r in out["rows"]] == [None, None, -1e5] and [r["entropy"] for r in out["rows"]] == [0.5, None, 1.0]
+    assert [r["top"] for r in out["rows"]] == [[[3, -0.25], [4, None]], [[3, None], [4, None]], []]
 
 
 # ---------------------------------------------------------------------------------------------- scheduler
