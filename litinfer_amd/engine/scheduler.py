@@ -147,9 +147,11 @@ class Scheduler:
             row_tile = int(getattr(engine, "row_tile", 1) or 1)
         if max_batch_tokens <= 0 or chunk_size <= 0 or row_tile <= 0:
             raise ValueError("scheduler: max_batch_tokens, chunk_size and row_tile must be positive")
-        if cache_budget is not None and (cache_budget <= 0 or min(cache_slack, cache_first, cache_recent or 0) < 0 or not engine.rt.attention_mass):
-            raise ValueError("scheduler: a cache_budget is positive, cache_slack, cache_first and cache_recent are not negative, and the engine "
-                             "keeps attention weights (Engine(..., attention_mass=True))")
+        if cache_budget is not None and not (
+                all(isinstance(x, (int, np.integer)) and not isinstance(x, bool) for x in (cache_budget, cache_slack, cache_first, cache_recent or 0))
+                and cache_budget > 0 and min(cache_slack, cache_first, cache_recent or 0) >= 0 and engine.rt.attention_mass):
+            raise ValueError("scheduler: a cache_budget is positive, cache_slack, cache_first and cache_recent are not negative, all whole numbers, and "
+                             "the engine keeps attention weights (Engine(..., attention_mass=True))")
         self.engine = engine
         self.cache = engine.cache
         self.cache_budget = None if cache_budget is None else int(cache_budget)

@@ -16,6 +16,7 @@ import time
 from pathlib import Path
 from typing import Iterator, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..engine import Engine, Scheduler, StepEntry
@@ -45,6 +46,8 @@ class CausalLM:
         """cache_budget: cached tokens that a request is cut to when it has grown beyond (`Scheduler`); None keeps all."""
         if quantize is not None:
             raise NotImplementedError("quantized weights are not supported")
+        if cache_budget is not None and (isinstance(cache_budget, bool) or not isinstance(cache_budget, (int, np.integer)) or cache_budget <= 0):
+            raise ValueError(f"cache_budget must be a positive whole number, found {cache_budget!r}")
         self.model_path = Path(model_path)
         print(f"[litinfer_amd] loading {self.model_path} ({dtype}) ...", flush=True)
         self.engine = Engine.from_dir(self.model_path, dtype=dtype, device=device, page_size=page_size,

@@ -168,3 +168,23 @@ def test_what_a_windowed_request_holds_does_not_count_against_what_it_takes(boun
     need = np.full((2, len(sched.cache.groups)), 1000, dtype=np.int32)
     held = np.full_like(need, 3)
     assert (sched._at_a_time(need) == sched._at_a_time(need, held=held)).all()
+
+
+@pytest.mark.parametrize("bad", [dict(cache_budget=0.5), dict(cache_budget=24.0), dict(cache_budget=True), dict(cache_budget="24"), dict(cache_slack=1.5), dict(cache_first=2.0),
+                                 dict(cache_recent=0.5), dict(cache_recent=math.nan), dict(cache_budget=math.inf)])
+def test_budgets_that_are_no_whole_numbers_are_refused_before_anything_runs(bounded_ops, model, bad):
+    with pytest.raises(ValueError, match="cache_budget"):
+        Scheduler(engine(model, num_pages=20), **{"cache_budget": 16, **bad})
+
+
+@pytest.mark.parametrize("bad", [0, -3, 0.5, 24.0, True, "24"])
+def test_the_entry_point_refuses_such_a_budget_before_it_loads_anything(bounded_ops, tmp_path, bad):
+    with pytest.raises(ValueError, match="cache_budget"):
+        Qwen2(tmp_path / "nothing is here", device="cpu", cache_budget=bad)
+
+
+def test_budgets_of_numpy_are_whole_numbers_too(bounded_ops, model):
+    sched = Scheduler(engine(model, num_pages=20), chunk_size=16, cache_budget=np.int64(24), cache_slack=np.int32(8), cache_recent=np.int16(4))
+    rid = sched.add_request(text(100), 2)
+    sched.run_to_completion()
+    assert len(sched.output(rid)) == 2
