@@ -35,7 +35,7 @@ struct MassArgs {
 struct SegList {
     int n;                       // 0: segment i is the i-th, all of them, lengths from the device
     int seg[EV_LIST], start[EV_LIST], q[EV_LIST], ctx[EV_LIST];
-    int off[EV_LIST];            // where the segment's places begin among all
+    int off[EV_LIST];            // where the segment's places begin among all; of single tokens, where its scores begin in the workspace
 };
 
 static uint32_t inverse_of(int page_size) { return page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size); }
@@ -162,6 +162,12 @@ __device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x
 // of 300 keys, 14 heads on 2, 6.2 in one kernel.
 #define SG_KEYS 64                // keys of a wave
 #define SG_WAVES 4
+// Floats of workspace that the requests of a launch take together, unless one takes more by itself: a batch beyond that goes in several launches, one
+// after the other, which use it again.  (256 MiB: more work than fills the chip many times over.)
+#define SG_ROOM (1L << 26)
+
+// A request's scores [heads, 64 parts] and behind them the statistics [heads, parts] (maximum, sum), in whole 16 bytes.
+__host__ __device__ __forceinline__ long single_floats(int nh, int parts) { return ((long)nh * parts * (SG_KEYS + 2) + 3) / 4 * 4; }
 
 // Scores of the 64 keys from k0 on against the heads of a kv head, 16 at a time, by a wave, and the maximum and sum for every head:
 // scores [head of the kv head, stride] from key k0 on, stats [head, parts].
@@ -229,17 +235,35 @@ __device__ __forceinline__ void single_scores(const T* __restrict__ qrow, const 
     }
 }
 
-// grid: x runs of 64 keys / 4, y kv heads, z requests; scores [request, nh, stride], stats [request, nh, parts].
+// Where a request's scores lie: those that are listed side by side, each as long as it is; others, from segment `first` on, `parts` runs of 64 each.
+struct Single {
+    int seg, ctx, parts;
+    float* scores;
+    float2* stats;
+};
+__device__ __forceinline__ Single single_of(const MassArgs& a, const SegList& list, int req, int first, int parts, float* work) {
+    Single s;
+    s.seg = list.n ? list.seg[req] : first + req;
+    s.ctx = list.n ? list.ctx[req] : device_ctx(a, s.seg, parts * SG_KEYS);
+    s.parts = list.n ? (s.ctx + SG_KEYS - 1) / SG_KEYS : parts;
+    s.scores = work + (list.n ? (long)list.off[req] : req * single_floats(a.nh, parts));
+    s.stats = reinterpret_cast<float2*>(s.scores + (size_t)a.nh * s.parts * SG_KEYS);
+    return s;
+}
+
+// grid: x runs of 64 keys / 4, y kv heads, z requests.
 template <typename T, int CH>
 __global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                           float* __restrict__ scores, long stride, float2* __restrict__ stats, int parts) {
-    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, rep = a.nh / a.nkv;
+                                                                           int first, float* __restrict__ work, int parts) {
+    const int req = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, rep = a.nh / a.nkv;
     const int k0 = (blockIdx.x * SG_WAVES + (threadIdx.x >> 6)) * SG_KEYS;
-    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, parts * SG_KEYS);
-    if (k0 >= ctx) return;
-    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
-    const size_t head0 = (size_t)req * a.nh + (size_t)kvh * rep;
-    single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)seg * a.max_blocks, kvh, k0, ctx, lane, scores + head0 * stride, stride, stats + head0 * parts, parts);
+    const Single s = single_of(a, list, req, first, parts, work);
+    if (k0 >= s.ctx) return;
+    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[s.seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    const size_t head0 = (size_t)kvh * rep;
+    const long stride = (long)s.parts * SG_KEYS;
+    single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)s.seg * a.max_blocks, kvh, k0, s.ctx, lane, s.scores + head0 * stride, stride, s.stats + head0 * s.parts,
+                         s.parts);
 }
 
 // lse of a head from the statistics of its `n` parts, by a wave.
@@ -291,27 +315,28 @@ __global__ __launch_bounds__(64 * block_waves(CH)) void mass_single_block_kernel
 }
 
 #define SG_LSE 64                 // heads of a kv head whose lse a block holds at a time
-__global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegList list, const float* __restrict__ scores, long stride,
-                                                              const float2* __restrict__ stats, int parts, float* __restrict__ mass) {
+__global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegList list, int first, float* __restrict__ work, int parts, float* __restrict__ mass) {
     __shared__ float lse[SG_LSE];
-    const int req = blockIdx.z, seg = list.n ? list.seg[req] : req, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, parts * SG_KEYS), t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
+    const int req = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
+    const Single s = single_of(a, list, req, first, parts, work);
+    const int ctx = s.ctx;
     if ((int)blockIdx.x * 256 >= ctx) return;
     const int n = (ctx + SG_KEYS - 1) / SG_KEYS;
-    const long row = t < ctx ? place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t) : -1;
+    const long row = t < ctx ? place_row(a, a.block_table + (size_t)s.seg * a.max_blocks, kvh, t) : -1;
     const float before = row >= 0 && !(a.fresh && t == ctx - 1) ? mass[row] : 0.f;
-    const size_t head0 = (size_t)req * a.nh + (size_t)kvh * rep;
+    const size_t head0 = (size_t)kvh * rep;
+    const long stride = (long)s.parts * SG_KEYS;
     float sum = 0.f;
     for (int h0 = 0; h0 < rep; h0 += SG_LSE) {
         const int heads = min(rep - h0, SG_LSE);
         __syncthreads();
         for (int h = w; h < heads; h += 4) {
-            const float v = join_stats(stats + (head0 + h0 + h) * parts, n, lane);
+            const float v = join_stats(s.stats + (head0 + h0 + h) * s.parts, n, lane);
             if (lane == 0) lse[h] = v;
         }
         __syncthreads();
         if (row >= 0)
-            for (int h = 0; h < heads; ++h) sum += __builtin_amdgcn_exp2f(scores[(head0 + h0 + h) * stride + t] - lse[h]);
+            for (int h = 0; h < heads; ++h) sum += __builtin_amdgcn_exp2f(s.scores[(head0 + h0 + h) * stride + t] - lse[h]);
     }
     if (row >= 0) mass[row] = before + sum;
 }
@@ -746,12 +771,12 @@ __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list
 struct MassPlan {
     int single = 0, multi = 0;           // segments of one token, of more
     int device_ctx = 0, multi_ctx = 0, multi_q = 0;
-    long stride = 0;                     // keys of a head's scores
-    int parts = 0, block_lds = 0;
+    int parts = 0, block_lds = 0;        // runs of 64 keys of the longest of them
     bool one_block = false;              // short contexts of single tokens: one kernel
+    bool listed = false;                 // single tokens are named in the launch, with their lengths
     int row_splits = 1, key_splits = 1, row_st = 1, key_st = 1, row_share = 1, key_share = 1, stage = 64;      // (shares: stages, pairs)
     long places = 0;                     // of the longer segments' sums, all together
-    long scores = 0, stats = 0, rows = 0, lse = 0, sums = 0, floats = 0;       // offsets, and the whole
+    long rows = 0, lse = 0, sums = 0, floats = 0;                              // offsets, and the whole (single tokens' scores lie first)
     bool tiled = false, valid = false;
 };
 
@@ -765,6 +790,32 @@ static bool tiled_takes(int dtype, int dh, int q_row_stride, const void* q, cons
 
 // Places of a segment's sums: whole blocks of keys.
 static long places_of(int ctx) { return (ctx + 64 * PT_WAVES - 1) / (64 * PT_WAVES) * (64L * PT_WAVES); }
+
+// The requests of the next launch of single tokens, from segment i on (which moves behind them): as many as a list and SG_ROOM hold.
+struct Singles { int n, parts; long floats; };
+static Singles next_singles(const int* q_len, const int* ctx_len, int nseg, int nh, int& i, SegList* list = nullptr, const int* q_start = nullptr) {
+    Singles s = {0, 0, 0};
+    for (; i < nseg && s.n < EV_LIST; ++i) {
+        if (q_len[i] != 1) continue;
+        const int parts = (ctx_len[i] + SG_KEYS - 1) / SG_KEYS;
+        const long mine = single_floats(nh, parts);
+        if (s.n && s.floats + mine > SG_ROOM) break;
+        if (list) {
+            list->seg[s.n] = i; list->start[s.n] = q_start[i]; list->q[s.n] = 1; list->ctx[s.n] = ctx_len[i]; list->off[s.n] = (int)s.floats;
+        }
+        s.parts = std::max(s.parts, parts);
+        s.floats += mine;
+        ++s.n;
+    }
+    if (list) list->n = s.n;
+    return s;
+}
+// The same where the lengths are read on the device: up to `left` requests of `parts` runs each.
+static Singles next_singles(int left, int parts, int nh) {
+    const long mine = single_floats(nh, parts);
+    const int n = (int)std::min((long)left, std::max(SG_ROOM / mine, 1L));
+    return {n, parts, n * mine};
+}
 
 static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int tokens, int padded_ctx, int nh, int nkv, int dh, bool f32, bool tiled) {
     MassPlan p;
@@ -790,16 +841,17 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
     if (!tiled) { p.floats = (long)tokens * nh; return p; }
     if (p.single) {
         p.parts = (p.device_ctx + SG_KEYS - 1) / SG_KEYS;
-        p.stride = (long)p.parts * SG_KEYS;
-        const long lds = 4 * (rep * p.stride + 2L * rep * p.parts + rep);
+        const long lds = 4 * (rep * (SG_KEYS + 2L) * p.parts + rep);
         // One kernel where a block has few keys, or where the blocks fill the compute units, us: bfloat16, 28 heads on 4 of 128, one request of 300 keys 9.0
         // (two kernels) and 6.8, 64 requests 13.3 and 7.1, of 1,000 20.0 and 14.8, of 2,000 32.5 and 25.6; 8 requests of 1,000 9.4 and 12.8, 64
         // of 2,000 on 2 kv heads 20.3 and 23.5.
         p.one_block = lds <= 150 * 1024 && (p.device_ctx <= 512 || ((long)p.single * nkv >= 192 && p.device_ctx <= 2048));
         p.block_lds = (int)lds;
-        p.scores = 0;
-        p.stats = p.one_block ? 0 : (long)p.single * nh * p.stride;
-        p.floats = p.one_block ? 0 : p.stats + 2L * p.single * nh * p.parts;
+        // a mix, or few: they are named, and their lengths need no trip to memory
+        p.listed = padded_ctx <= 0 && (p.single < nseg || nseg <= EV_LIST);
+        if (!p.one_block && !p.listed) p.floats = next_singles(p.single, p.parts, nh).floats;
+        if (!p.one_block && p.listed)
+            for (int i = 0; i < nseg;) p.floats = std::max(p.floats, next_singles(q_len, ctx_len, nseg, nh, i).floats);
     }
     if (p.multi) {
         // Blocks of about equal length: as many as the compute units hold at a time, each with no less than 8 stages of keys (4 pairs of a head and a stage
@@ -865,7 +917,7 @@ static bool allow_lds(K kernel, int bytes) {
 }
 
 template <typename T, int DHP>
-static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, bool padded,
+static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b,
                              int nseg, int tokens, float* work, hipStream_t stream) {
     constexpr int PE = 16 / sizeof(T), CH16 = DHP / (4 * PE), ST = sizeof(T) == 2 ? 2 : 1;
     constexpr int LDS_BYTES = PT_BUFS * 32 * stage_tiles(DHP * (int)sizeof(T)) * DHP * (int)sizeof(T);
@@ -873,28 +925,18 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
         for (int at = 0, i = 0; at < p.single;) {
             SegList list;
             list.n = 0;
-            int n = p.single;
-            if (p.single < nseg || (!padded && nseg <= EV_LIST)) {   // a mix, or few: they are named, and their lengths need no trip to memory
-                n = 0;
-                for (; i < nseg && n < EV_LIST; ++i)
-                    if (b.q_len[i] == 1) {
-                        list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = 1; list.ctx[n] = b.ctx_len[i]; list.off[n++] = 0;
-                    }
-                list.n = n;
-            }
+            const Singles now = p.listed ? next_singles(b.q_len, b.ctx_len, nseg, a.nh, i, &list, b.q_start)
+                                : p.one_block ? Singles{p.single, p.parts, 0} : next_singles(p.single - at, p.parts, a.nh);
             if (p.one_block) {
                 const auto block = mass_single_block_kernel<T, CH16>;
                 if (!allow_lds(block, p.block_lds)) return LI_ERR_LAUNCH;
-                block<<<dim3(a.nkv, n), 64 * block_waves(CH16), p.block_lds, stream>>>(q, k, a, list, (int)p.stride, mass);
-                at += n;
-                continue;
+                block<<<dim3(a.nkv, now.n), 64 * block_waves(CH16), p.block_lds, stream>>>(q, k, a, list, p.parts * SG_KEYS, mass);
+            } else {
+                mass_single_scores_kernel<T, CH16><<<dim3((now.parts + SG_WAVES - 1) / SG_WAVES, a.nkv, now.n), 64 * SG_WAVES, 0, stream>>>(
+                    q, k, a, list, at, work, now.parts);
+                mass_single_add_kernel<<<dim3((now.parts + 3) / 4, a.nkv, now.n), 256, 0, stream>>>(a, list, at, work, now.parts, mass);
             }
-            float* scores = work + p.scores + (size_t)at * a.nh * p.stride;
-            float2* stats = (float2*)(work + p.stats) + (size_t)at * a.nh * p.parts;
-            mass_single_scores_kernel<T, CH16><<<dim3((p.parts + SG_WAVES - 1) / SG_WAVES, a.nkv, n), 64 * SG_WAVES, 0, stream>>>(
-                q, k, a, list, scores, p.stride, stats, p.parts);
-            mass_single_add_kernel<<<dim3((p.device_ctx + 255) / 256, a.nkv, n), 256, 0, stream>>>(a, list, scores, p.stride, stats, p.parts, mass);
-            at += n;
+            at += now.n;
         }
     }
     if (p.multi) {
@@ -934,11 +976,11 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
 }
 
 template <typename T>
-static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, bool padded, int nseg, int tokens,
+static int launch_mass(const T* q, const T* k, float* mass, const MassArgs& a, const MassPlan& p, const Batch& b, int nseg, int tokens,
                        float* work, hipStream_t stream) {
-    if (p.tiled && a.dh <= 64) return launch_mass_tiled<T, 64>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
-    if (p.tiled && a.dh <= 128) return launch_mass_tiled<T, 128>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
-    if (p.tiled) return launch_mass_tiled<T, 256>(q, k, mass, a, p, b, padded, nseg, tokens, work, stream);
+    if (p.tiled && a.dh <= 64) return launch_mass_tiled<T, 64>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    if (p.tiled && a.dh <= 128) return launch_mass_tiled<T, 128>(q, k, mass, a, p, b, nseg, tokens, work, stream);
+    if (p.tiled) return launch_mass_tiled<T, 256>(q, k, mass, a, p, b, nseg, tokens, work, stream);
     mass_rows_kernel<T><<<dim3(p.multi_q, a.nh, nseg), 64, 0, stream>>>(q, k, a, work);
     mass_keys_kernel<T><<<dim3((p.multi_ctx + 63) / 64, a.nkv, nseg), 256, 0, stream>>>(q, k, a, work, mass);
     return li_launch_status();
@@ -965,8 +1007,8 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
     const MassPlan p = mass_plan(h_q_len, h_ctx_len, nseg, tokens, padded_ctx, nh, nkv, dh, dtype == LI_F32, tiled_takes(dtype, dh, q_row_stride, q, kc, scale, tokens, nh, (long)num_pages * nkv * page_size));
     if (!p.valid || p.floats > work_floats) return LI_ERR_SIZE;
     const Batch b = {h_q_start, h_q_len, h_ctx_len};
-    if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, padded_ctx > 0, nseg, tokens, work, stream);
-    return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, padded_ctx > 0, nseg, tokens, work, stream);
+    if (dtype == LI_F32) return launch_mass((const float*)q, (const float*)kc, mass, a, p, b, nseg, tokens, work, stream);
+    return launch_mass((const bf16_t*)q, (const bf16_t*)kc, mass, a, p, b, nseg, tokens, work, stream);
 }
 
 // ------------------------------------------------------------------ which keys stay

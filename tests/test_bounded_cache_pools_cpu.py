@@ -188,3 +188,36 @@ def test_budgets_of_numpy_are_whole_numbers_too(bounded_ops, model):
     rid = sched.add_request(text(100), 2)
     sched.run_to_completion()
     assert len(sched.output(rid)) == 2
+
+
+# ---------------------------------------------------------------------------------------------- workspace
+def work_floats(q_len, ctx_len, nh, nkv, dh=64, padded=0):
+    q, c = np.asarray(q_len, dtype=np.int32), np.asarray(ctx_len, dtype=np.int32)
+    return ops._mass_work_floats()(q.ctypes.data, c.ctypes.data, len(q), int(q.sum()), padded, nh, nkv, dh, ops._DT[torch.bfloat16], (nh + 2 * nkv) * dh, 1 << 20, 1 << 20,
+                                   0.125, 1 << 20)
+
+
+ROOM = 1 << 26                                                    # floats that requests take together
+
+
+def scores(nh, ctx):
+    """What a request's scores and statistics take, in whole 16 bytes."""
+    return -(-nh * -(-ctx // 64) * 66 // 4) * 4
+
+
+def test_the_workspace_of_single_tokens_goes_by_what_each_has_cached():
+    ctx = [100] * 63 + [32000]
+    assert work_floats([1] * 64, ctx, 28, 4) == sum(scores(28, c) for c in ctx) < 1.1 * 28 * sum(ctx) * 66 / 64
+    assert work_floats([1, 40, 1], [500, 90, 70000], 28, 4) - work_floats([40], [90], 28, 4) <= scores(28, 500) + scores(28, 70000) + 4096
+
+
+@pytest.mark.parametrize("n,nh,nkv,longest", [(64, 40, 8, 32768), (256, 40, 8, 131072), (1000, 28, 4, 4096), (3, 64, 8, 1 << 20)])
+def test_the_workspace_of_single_tokens_has_a_bound(n, nh, nkv, longest):
+    most = max(ROOM, scores(nh, longest))
+    assert work_floats([1] * n, [9] * n, nh, nkv, padded=longest) <= most               # a recorded step: any length up to the tables'
+    assert work_floats([1] * n, [longest] * n, nh, nkv) <= most
+
+
+def test_the_workspace_of_a_request_that_takes_more_than_the_room_by_itself():
+    assert work_floats([1] * 3, [5000, 4 << 20, 5000], 64, 8) == scores(64, 4 << 20) > ROOM
+    assert work_floats([1] * 3, [9] * 3, 64, 8, padded=4 << 20) == scores(64, 4 << 20)
