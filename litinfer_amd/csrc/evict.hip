@@ -32,10 +32,13 @@ struct MassArgs {
 // Segments of the batch that a launch takes, by value: a step's mix is known on the host, and what the workspace was laid out for is what the
 // kernels go by.  (A recorded step has single tokens only, all of them, and reads their contexts from the device.)
 #define EV_LIST 64
+struct Seg {
+    int seg, start, q, ctx;
+    int off;                     // where the segment's places begin among all; of single tokens, where its scores begin in the workspace
+};
 struct SegList {
     int n;                       // 0: segment i is the i-th, all of them, lengths from the device
-    int seg[EV_LIST], start[EV_LIST], q[EV_LIST], ctx[EV_LIST];
-    int off[EV_LIST];            // where the segment's places begin among all; of single tokens, where its scores begin in the workspace
+    Seg of[EV_LIST];             // (a segment's numbers side by side: a trip to the launch's arguments takes long)
 };
 
 static uint32_t inverse_of(int page_size) { return page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)page_size); }
@@ -237,16 +240,24 @@ __device__ __forceinline__ void single_scores(const T* __restrict__ qrow, const 
 
 // Where a request's scores lie: those that are listed side by side, each as long as it is; others, from segment `first` on, `parts` runs of 64 each.
 struct Single {
-    int seg, ctx, parts;
+    int seg, start, ctx, parts;
     float* scores;
     float2* stats;
 };
 __device__ __forceinline__ Single single_of(const MassArgs& a, const SegList& list, int req, int first, int parts, float* work) {
     Single s;
-    s.seg = list.n ? list.seg[req] : first + req;
-    s.ctx = list.n ? list.ctx[req] : device_ctx(a, s.seg, parts * SG_KEYS);
-    s.parts = list.n ? (s.ctx + SG_KEYS - 1) / SG_KEYS : parts;
-    s.scores = work + (list.n ? (long)list.off[req] : req * single_floats(a.nh, parts));
+    if (list.n) {
+        const Seg of = list.of[req];
+        s.seg = of.seg; s.start = of.start; s.ctx = of.ctx;
+        s.parts = (of.ctx + SG_KEYS - 1) / SG_KEYS;
+        s.scores = work + of.off;
+    } else {
+        s.seg = first + req;
+        s.start = a.q_start[s.seg];
+        s.ctx = device_ctx(a, s.seg, parts * SG_KEYS);
+        s.parts = parts;
+        s.scores = work + req * single_floats(a.nh, parts);
+    }
     s.stats = reinterpret_cast<float2*>(s.scores + (size_t)a.nh * s.parts * SG_KEYS);
     return s;
 }
@@ -259,7 +270,7 @@ __global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const
     const int k0 = (blockIdx.x * SG_WAVES + (threadIdx.x >> 6)) * SG_KEYS;
     const Single s = single_of(a, list, req, first, parts, work);
     if (k0 >= s.ctx) return;
-    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[s.seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    const T* qrow = q + (size_t)s.start * a.q_row_stride + (size_t)kvh * rep * a.dh;
     const size_t head0 = (size_t)kvh * rep;
     const long stride = (long)s.parts * SG_KEYS;
     single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)s.seg * a.max_blocks, kvh, k0, s.ctx, lane, s.scores + head0 * stride, stride, s.stats + head0 * s.parts,
@@ -288,13 +299,13 @@ __global__ __launch_bounds__(64 * block_waves(CH)) void mass_single_block_kernel
                                                                           float* __restrict__ mass) {
     constexpr int WAVES = block_waves(CH);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int req = blockIdx.y, seg = list.n ? list.seg[req] : req, kvh = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, rep = a.nh / a.nkv;
-    const int ctx = list.n ? list.ctx[req] : device_ctx(a, seg, stride), parts = stride / SG_KEYS;
+    const int req = blockIdx.y, seg = list.n ? list.of[req].seg : req, kvh = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6, rep = a.nh / a.nkv;
+    const int ctx = list.n ? list.of[req].ctx : device_ctx(a, seg, stride), parts = stride / SG_KEYS;
     float* scores = reinterpret_cast<float*>(lds);
     float2* stats = reinterpret_cast<float2*>(scores + (size_t)rep * stride);
     float* lse = reinterpret_cast<float*>(stats + rep * parts);
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
-    const T* qrow = q + (size_t)(list.n ? list.start[req] : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    const T* qrow = q + (size_t)(list.n ? list.of[req].start : a.q_start[seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
     for (int k0 = w * SG_KEYS; k0 < ctx; k0 += WAVES * SG_KEYS)
         single_scores<T, CH>(qrow, k, a, table, kvh, k0, ctx, lane, scores, stride, stats, parts);
     __syncthreads();
@@ -441,9 +452,9 @@ __global__ __launch_bounds__(64 * PT_WAVES) void mass_rows_tile_kernel(const T* 
                                                                        int tokens) {
     constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int which = blockIdx.z / splits, seg = list.seg[which], split = blockIdx.z % splits, kvh = blockIdx.x % a.nkv, tok0 = list.start[which];
+    const int which = blockIdx.z / splits, seg = list.of[which].seg, split = blockIdx.z % splits, kvh = blockIdx.x % a.nkv, tok0 = list.of[which].start;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
-    const int nq = list.q[which], base = list.ctx[which] - nq, rep = a.nh / a.nkv, pieces = a.dh / PE;
+    const int nq = list.of[which].q, base = list.of[which].ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE;
     const int tiles = (nq + 32 * ST - 1) / (32 * ST), wt0 = blockIdx.x / a.nkv * PT_WAVES;
     if (wt0 >= tiles * rep) return;
     const int* table = a.block_table + (size_t)seg * a.max_blocks;
@@ -605,7 +616,7 @@ __global__ __launch_bounds__(256) void mass_lse_kernel(const float2* __restrict_
 // The columns' sums: a wave holds ST * 32 keys, the block streams the queries that see any of them, head by head.
 // grid: x kv heads times blocks of keys (of the longest segment), y splits of the (head, stage of queries) pairs, z segments.  A block of keys has
 // as many splits as make about `share` pairs each: late keys are seen by few queries.
-// part [splits, kv heads, places]; a segment's places begin at list.off.
+// part [splits, kv heads, places]; a segment's places begin at its `off`.
 // The pairs of the block of keys from b0 on: its first stage of queries, stages a head, splits.
 struct Pairs { int first, n, splits; };
 __device__ __forceinline__ Pairs pairs_of(int b0, int base, int nq, int rep, int rows, int share) {
@@ -619,9 +630,9 @@ __global__ __launch_bounds__(64 * PT_WAVES, DHP * sizeof(T) <= 256 ? 2 : 1) void
     constexpr int PE = 16 / sizeof(T), PPR = DHP / PE, CH = PPR / 2, TPS = stage_tiles(16 * PPR), ROWS = 32 * TPS, STAGE_BYTES = ROWS * PPR * 16, KEYS = 32 * ST;
     constexpr int LOADS = ROWS * PPR / (64 * PT_WAVES);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int which = blockIdx.z, seg = list.seg[which], kvh = blockIdx.x % a.nkv, split = blockIdx.y;
+    const int which = blockIdx.z, seg = list.of[which].seg, kvh = blockIdx.x % a.nkv, split = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, half = lane >> 5;
-    const int nq = list.q[which], ctx = list.ctx[which], base = ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE, tok0 = list.start[which];
+    const int nq = list.of[which].q, ctx = list.of[which].ctx, base = ctx - nq, rep = a.nh / a.nkv, pieces = a.dh / PE, tok0 = list.of[which].start;
     const int b0 = blockIdx.x / a.nkv * KEYS * PT_WAVES, k0 = b0 + w * KEYS;
     if (b0 >= ctx) return;
     const Pairs pairs = pairs_of(b0, base, nq, rep, ROWS, share);
@@ -736,7 +747,7 @@ __global__ __launch_bounds__(64 * PT_WAVES, DHP * sizeof(T) <= 256 ? 2 : 1) void
         if (steps & 1) add_up(acc[0], lacc[0], j);
         else add_up(acc[1], lacc[1], j);
     }
-    float* out = part + ((size_t)split * a.nkv + kvh) * places + list.off[blockIdx.z];
+    float* out = part + ((size_t)split * a.nkv + kvh) * places + list.of[blockIdx.z].off;
 #pragma unroll
     for (int x = 0; x < ST; ++x)
 #pragma unroll
@@ -751,12 +762,12 @@ __global__ __launch_bounds__(64 * PT_WAVES, DHP * sizeof(T) <= 256 ? 2 : 1) void
 // The splits' sums, in their order, join the keys'.
 __global__ __launch_bounds__(256) void mass_join_kernel(MassArgs a, SegList list, const float* __restrict__ part, int keys, int rows, int share, long places,
                                                         float* __restrict__ mass) {
-    const int seg = list.seg[blockIdx.z], kvh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = list.ctx[blockIdx.z];
+    const int seg = list.of[blockIdx.z].seg, kvh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = list.of[blockIdx.z].ctx;
     if (t >= ctx) return;
     const long row = place_row(a, a.block_table + (size_t)seg * a.max_blocks, kvh, t);
     if (row < 0) return;
-    const int nq = list.q[blockIdx.z], splits = pairs_of(t / keys * keys, ctx - nq, nq, a.nh / a.nkv, rows, share).splits;
-    const float* src = part + (size_t)kvh * places + list.off[blockIdx.z] + t;
+    const int nq = list.of[blockIdx.z].q, splits = pairs_of(t / keys * keys, ctx - nq, nq, a.nh / a.nkv, rows, share).splits;
+    const float* src = part + (size_t)kvh * places + list.of[blockIdx.z].off + t;
     float sum = 0.f;
     for (int s = 0; s < splits; s += 4) {                // (four on their way at a time)
         float v[4];
@@ -800,9 +811,7 @@ static Singles next_singles(const int* q_len, const int* ctx_len, int nseg, int 
         const int parts = (ctx_len[i] + SG_KEYS - 1) / SG_KEYS;
         const long mine = single_floats(nh, parts);
         if (s.n && s.floats + mine > SG_ROOM) break;
-        if (list) {
-            list->seg[s.n] = i; list->start[s.n] = q_start[i]; list->q[s.n] = 1; list->ctx[s.n] = ctx_len[i]; list->off[s.n] = (int)s.floats;
-        }
+        if (list) list->of[s.n] = {i, q_start[i], 1, ctx_len[i], (int)s.floats};
         s.parts = std::max(s.parts, parts);
         s.floats += mine;
         ++s.n;
@@ -955,7 +964,7 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                 int n = 0;
                 for (; i < nseg && n < EV_LIST; ++i)
                     if (b.q_len[i] > 1) {
-                        list.seg[n] = i; list.start[n] = b.q_start[i]; list.q[n] = b.q_len[i]; list.ctx[n] = b.ctx_len[i]; list.off[n++] = (int)off;
+                        list.of[n++] = {i, b.q_start[i], b.q_len[i], b.ctx_len[i], (int)off};
                         off += places_of(b.ctx_len[i]);
                     }
                 list.n = n;
