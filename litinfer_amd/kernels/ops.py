@@ -2042,7 +2042,9 @@ def _mass_plan(qkv, k, meta, nh: int, nkv: int, dh: int, page_size: int, scale: 
     dt, hs, hq, hc = _DT[qkv.dtype], hs.ctypes.data, hq.ctypes.data, hc.ctypes.data
     need = int(_mass_work_floats()(hq, hc, n, t, padded, nh, nkv, dh, dt, qkv.stride(0), qkv.data_ptr(), k.data_ptr(), float(scale), k.shape[0] * nkv * page_size))
     _chk(need >= 0, "attention_mass: the segments' lengths are not those of a batch")
-    return (need, (dt, bt.data_ptr(), meta.max_blocks), (meta.q_start.data_ptr(), meta.q_len.data_ptr(), meta.ctx_len.data_ptr(), hs, hq, hc),
+    # (one of eight sizes between two powers of two: every batch of another size would be a view that the workspace keeps)
+    step = 1 << max(need.bit_length() - 4, 8)
+    return (-(-need // step) * step, (dt, bt.data_ptr(), meta.max_blocks), (meta.q_start.data_ptr(), meta.q_len.data_ptr(), meta.ctx_len.data_ptr(), hs, hq, hc),
             (n, t, padded, nh, nkv, dh, page_size, k.shape[0]))
 
 

@@ -11,6 +11,7 @@ import helpers
 import plain_impl
 from litinfer_amd.cache import CacheFull
 from litinfer_amd.engine import Engine, Scheduler
+from litinfer_amd.engine.workspace import Workspace
 from litinfer_amd.kernels import ops
 from litinfer_amd.models import Qwen2
 from litinfer_amd.sampling import Sampler, TokenLogprob
@@ -221,3 +222,20 @@ def test_the_workspace_of_single_tokens_has_a_bound(n, nh, nkv, longest):
 def test_the_workspace_of_a_request_that_takes_more_than_the_room_by_itself():
     assert work_floats([1] * 3, [5000, 4 << 20, 5000], 64, 8) == scores(64, 4 << 20) > ROOM
     assert work_floats([1] * 3, [9] * 3, 64, 8, padded=4 << 20) == scores(64, 4 << 20)
+
+
+def test_batches_of_many_sizes_ask_the_workspace_for_few(monkeypatch):
+    monkeypatch.setattr(ops, "_here", lambda what, *ts: None)
+    asked = []
+    monkeypatch.setattr(ops, "_run", lambda module, name, *args: asked.append(args))
+    ws, rng = Workspace("cpu"), np.random.default_rng(3)
+    for _ in range(400):
+        segs = [(int(q), int(q + c)) for q, c in zip(rng.choice([1, 1, 1, 7, 40], 5), rng.integers(0, 3000, 5))]
+        meta, pages = cases.batch(segs, 16, "cpu")
+        ops.attention_mass(torch.zeros(meta.num_tokens, 12 * 64), torch.zeros(pages, 2, 16, 1), torch.zeros(pages, 2, 16, 64), meta, 8, 2, 64, 16, 0.125, ws=ws)
+    sizes = [args[-1] for args in asked]
+    needs = [work for work in sizes if work > 0]
+    assert len(asked) == len(needs) == 400
+    # eight sizes between two powers of two, and an eighth more at most
+    octaves = math.log2(max(sizes) / min(sizes)) + 1
+    assert len(ws._views) <= len(set(sizes)) <= 8 * octaves + 1 and ws.generation <= 2 * octaves
