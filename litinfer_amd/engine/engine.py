@@ -157,6 +157,13 @@ class Engine:
                 out[groups.index(paged)] += paged.bytes_per_token(self.rt.dtype) * self.page_size
         return out
 
+    def _page_memory(self, free: int) -> int:
+        """Of `free` bytes, those that the pages may take: the rest is for a step's buffers.  What the sums of attention weight take at most (256 MiB, of
+        which an older buffer and one half as large again may be held while it grows) is set aside first: to run out there, in the middle of a
+        forward, would leave some layers' sums added to."""
+        aside = 5 << 27 if self.rt.attention_mass else 0
+        return int(max(free - aside, free // 2) * 0.85)
+
     def _make_cache(self) -> None:
         """The pools' sizes.  Given `num_pages` (a number for every group, or one per group),
         `max_tokens` or LLAISYS_NUM_BLOCKS, every group gets that many pages.  Otherwise the memory
@@ -185,7 +192,7 @@ class Engine:
             if self.rt.device.type == "cuda" and groups:
                 free, _ = torch.cuda.mem_get_info(self.rt.device)
                 bpp = [max(1, b) for b in self._group_page_bytes()]
-                budget = int(free * 0.85)
+                budget = self._page_memory(free)
                 windowed = sum(n * b for n, b, g in zip(pages, bpp, groups) if g.reach > 0)
                 if windowed > budget // 2:                # (windows as long as the contexts: no group is small)
                     share = max(1, budget // sum(bpp))

@@ -234,8 +234,16 @@ def test_batches_of_many_sizes_ask_the_workspace_for_few(monkeypatch):
         meta, pages = cases.batch(segs, 16, "cpu")
         ops.attention_mass(torch.zeros(meta.num_tokens, 12 * 64), torch.zeros(pages, 2, 16, 1), torch.zeros(pages, 2, 16, 64), meta, 8, 2, 64, 16, 0.125, ws=ws)
     sizes = [args[-1] for args in asked]
-    needs = [work for work in sizes if work > 0]
-    assert len(asked) == len(needs) == 400
+    assert len(sizes) == 400
     # eight sizes between two powers of two, and an eighth more at most
     octaves = math.log2(max(sizes) / min(sizes)) + 1
     assert len(ws._views) <= len(set(sizes)) <= 8 * octaves + 1 and ws.generation <= 2 * octaves
+
+
+def test_what_the_sums_take_is_set_aside_before_the_pages_are_counted(bounded_ops, model):
+    a, b = engine(model, num_pages=10), engine(model, num_pages=10, attention_mass=False)
+    free = 200 << 30
+    assert b._page_memory(free) == int(free * 0.85)
+    # (the buffer that is too small and the one that takes its place: 4 bytes a float, grown by half)
+    assert a._page_memory(free) <= 0.85 * (free - 4 * (ROOM + ROOM * 3 // 2)) and a._page_memory(free) > 0.84 * free
+    assert a._page_memory(1 << 30) == int((1 << 29) * 0.85)
