@@ -15,6 +15,8 @@
 #include <type_traits>
 
 #define EV_MAX_DH 256
+// Places of a request, and rows that a list has room for: loops that step over them in 32 bits end behind the last.
+#define EV_MAX_PLACES (1L << 30)
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -1004,7 +1006,7 @@ extern "C" int li_attention_mass(const void* q, int q_row_stride, const void* kc
                                  int padded_ctx, int nh, int nkv, int dh, int page_size, int num_pages, float scale, int fresh, float* work,
                                  long work_floats, hipStream_t stream) {
     if (nseg <= 0 || nseg > 65535 || tokens <= 0 || nh <= 0 || nh > 65535 || nkv <= 0 || nkv > 4095 || nh % nkv || dh <= 0 || dh > EV_MAX_DH || page_size <= 0 ||
-        max_blocks <= 0 || (long)max_blocks * page_size >= 1L << 31 || num_pages <= 0 ||
+        max_blocks <= 0 || (long)max_blocks * page_size > EV_MAX_PLACES || num_pages <= 0 ||
         (long)num_pages * nkv * page_size >= 1L << 31 || !h_q_start || !h_q_len || !h_ctx_len || !work)
         return LI_ERR_SIZE;
     const long room = (long)max_blocks * page_size;
@@ -1290,8 +1292,8 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_long_kernel(SelectArgs a)
 // mass [entries, num_pages, nkv, page_size]; lens, keeps [n]; out [entries, n, nkv, K], ascending, -1 behind the last.
 extern "C" int li_evict_select(const float* mass, const int* block_table, int max_blocks, const int* lens, const int* keeps, int n, int first, int recent,
                                int* out, int K, int entries, int nkv, int page_size, int num_pages, hipStream_t stream) {
-    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || first < 0 || recent < 0 || max_blocks <= 0 || num_pages <= 0 || page_size <= 0 ||
-        (long)max_blocks * page_size >= 1L << 31)
+    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || K > EV_MAX_PLACES || first < 0 || recent < 0 || max_blocks <= 0 || num_pages <= 0 || page_size <= 0 ||
+        (long)max_blocks * page_size > EV_MAX_PLACES)
         return LI_ERR_SIZE;
     const SelectArgs a = {mass, block_table, lens, keeps, max_blocks, first, recent, K, nkv, page_size, num_pages, inverse_of(page_size), out,
                           page_size % 4 == 0 && (uintptr_t)mass % 16 == 0};
@@ -1409,8 +1411,8 @@ __global__ __launch_bounds__(CMP_NT, 6) void cache_compact_kernel(CompactTensors
 // [entries, n, nkv, K] as li_evict_select leaves it.
 extern "C" int li_cache_compact(void* const* tensors, const int* row_bytes, int count, const int* block_table, int max_blocks, const int* kept, int K, int n,
                                 int entries, int nkv, int page_size, int num_pages, hipStream_t stream) {
-    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || count <= 0 || count > CMP_MAX_TENSORS || max_blocks <= 0 ||
-        num_pages <= 0 || page_size <= 0 || (long)max_blocks * page_size >= 1L << 31)
+    if (n <= 0 || n > 65535 || entries <= 0 || entries > 65535 || nkv <= 0 || K <= 0 || K > EV_MAX_PLACES || count <= 0 || count > CMP_MAX_TENSORS || max_blocks <= 0 ||
+        num_pages <= 0 || page_size <= 0 || (long)max_blocks * page_size > EV_MAX_PLACES)
         return LI_ERR_SIZE;
     CompactTensors ts = {};
     for (int i = 0; i < count; ++i) {

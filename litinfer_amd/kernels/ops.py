@@ -2032,6 +2032,9 @@ def _mass_plan(qkv, k, meta, nh: int, nkv: int, dh: int, page_size: int, scale: 
     _chk(all(x.dtype is torch.int32 and x.numel() == n and x.is_contiguous() for x in (meta.q_start, meta.q_len, meta.ctx_len)),
          "attention_mass: q_start, q_len and ctx_len must be int32 [segments]")
     _chk(meta.max_blocks * page_size >= meta.max_ctx_len, "attention_mass: block table too short")
+    _chk(meta.max_blocks * page_size <= EVICT_MAX_PLACES, "attention_mass: more than 2^30 places a request")
+    _chk(k.shape[0] * nkv * page_size < 1 << 31, "attention_mass: 2^31 rows or more in the pool")
+    _chk(qkv.stride(0) < 1 << 31, "attention_mass: rows of qkv 2^31 elements apart or more")
     if not t:
         return ()
     hs, hq, hc = meta.host_q_start, meta.host_q_len, meta.host_ctx_len
@@ -2052,10 +2055,14 @@ def _mass_work_floats():
     return _lib_fn("evict", "li_attention_mass_work_floats", [P, P] + [I] * 8 + [P, P, F, L], c_long)
 
 
-def _check_requests(what: str, block_table, n: int, page_size: int) -> None:
+EVICT_MAX_PLACES = 1 << 30             # of a request, and rows that a list has room for
+
+
+def _check_requests(what: str, block_table, n: int, page_size: int, pages: int, room: int) -> None:
     _chk(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n and block_table.shape[1] > 0
          and block_table.is_contiguous(), f"{what}: block_table must be int32 [requests, blocks]")
-    _chk(block_table.shape[1] * page_size < 1 << 31, f"{what}: more than 2^31 places a request")
+    _chk(block_table.shape[1] * page_size <= EVICT_MAX_PLACES and room <= EVICT_MAX_PLACES, f"{what}: more than 2^30 places a request")
+    _chk(pages < 1 << 31, f"{what}: 2^31 pages or more")
 
 
 def evict_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor, first: int, recent: int, out: torch.Tensor) -> None:
@@ -2063,17 +2070,17 @@ def evict_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tens
     than `out` has room for): the last `recent` of them, the first `first` (as far as these are not too many), and of the others those with the
     largest sums, the lower place first on ties (a sum of NaN after all others).  mass [entries, pages, kv_heads, page_size, 1] float32;
     block_table int32 [requests, blocks]; lens, keep int32 [requests]; out int32 [entries, requests, kv_heads, K]: the places in rising
-    order, -1 behind the last."""
+    order, -1 behind the last.  Up to 2^30 places a request and 2^30 rows a list (here and in `cache_compact` and `attention_mass`)."""
     _here("evict_select", mass, block_table, lens, keep, out)
     _chk(mass.dim() == 5 and mass.shape[4] == 1 and mass.dtype is torch.float32 and mass.is_contiguous(),
          "evict_select: mass must be float32 [entries, pages, kv_heads, page_size, 1]")
     entries, pages, nkv, page_size, _ = mass.shape
     n = lens.numel()
     _chk(all(x.dtype is torch.int32 and x.shape == (n,) and x.is_contiguous() for x in (lens, keep)), "evict_select: lens and keep must be int32 [requests]")
-    _check_requests("evict_select", block_table, n, page_size)
     _chk(first >= 0 and recent >= 0, "evict_select: first and recent must not be negative")
     _chk(out.dtype is torch.int32 and out.dim() == 4 and out.shape[:3] == (entries, n, nkv) and out.is_contiguous(),
          "evict_select: out must be int32 [entries, requests, kv_heads, K]")
+    _check_requests("evict_select", block_table, n, page_size, pages, out.shape[3])
     _chk(entries <= 65535 and n <= 65535, "evict_select: at most 65,535 entries and requests")
     if out.numel():
         _run("evict", "li_evict_select", mass.data_ptr(), block_table.data_ptr(), block_table.shape[1], lens.data_ptr(), keep.data_ptr(), n,
@@ -2098,7 +2105,8 @@ def cache_compact(tensors, block_table: torch.Tensor, kept: torch.Tensor) -> Non
              and t.shape[4] * t.element_size() % 4 == 0 for t in tensors),
          "cache_compact: tensors must be contiguous [entries, pages, kv_heads, page_size, size] with rows of whole 4 bytes")
     pages, _, page_size = tensors[0].shape[1:4]
-    _check_requests("cache_compact", block_table, n, page_size)
+    _check_requests("cache_compact", block_table, n, page_size, pages, most)
+    _chk(pages * nkv * page_size < 1 << 31, "cache_compact: 2^31 rows or more in the pool")
     _chk(entries <= 65535 and n <= 65535, "cache_compact: at most 65,535 entries and requests")
     if kept.numel() and all(t.numel() for t in tensors):
         count = len(tensors)
