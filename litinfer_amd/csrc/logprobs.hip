@@ -309,11 +309,11 @@ extern "C" int li_token_logprobs_max_vocab(void) { return LP_MAX_GROUPS * LP_GRO
 // outside the row has no probability (NaN).
 extern "C" int li_token_logprobs(const float* logits, long stride, const int* ids, int n, int V, int top, float* logprob, float* entropy,
                                  int* top_ids, float* top_logprob, float* work, hipStream_t stream) {
-    if (n <= 0 || V <= 0 || stride < V || groups_of(V) > LP_MAX_GROUPS || top < 0 || top > LP_MAX_TOP || top > V || !work) return LI_ERR_SIZE;
+    if (n <= 0 || n > 1 << 30 || V <= 0 || stride < V || groups_of(V) > LP_MAX_GROUPS || top < 0 || top > LP_MAX_TOP || top > V || !work) return LI_ERR_SIZE;
     const int u = share_groups(n), shares = row_shares(V, u), groups = groups_of(V);
     RowShare* share = (RowShare*)work;
     float* tops = work + 4L * n * shares;
-    for (int at = 0; at < n; at += 65535) {               // (rows are the grid's second axis)
+    for (int at = 0; at < n; at += 65535) {               // (rows are the first grid's second axis, and a launch has fewer than 2^32 threads)
         const int rows = n - at < 65535 ? n - at : 65535;
         const dim3 grid((shares + LP_WAVES - 1) / LP_WAVES, rows);
         const float* x = logits + (size_t)at * stride;
@@ -321,7 +321,9 @@ extern "C" int li_token_logprobs(const float* logits, long stride, const int* id
         float* g = top ? tops + (size_t)at * groups : nullptr;
         if (u == 2) logprob_rows_kernel<2><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
         else logprob_rows_kernel<8><<<grid, 64 * LP_WAVES, 0, stream>>>(x, stride, V, shares, s, g, groups);
+        logprob_join_kernel<<<rows, 64 * LP_JOIN_WAVES, top ? 4 * (groups + (top < groups ? top : groups) * LP_GROUP) : 0, stream>>>(
+            x, stride, V, shares, s, g, groups, ids + at, logprob + at, entropy + at, top, top ? top_ids + (size_t)at * top : nullptr,
+            top ? top_logprob + (size_t)at * top : nullptr);
     }
-    logprob_join_kernel<<<n, 64 * LP_JOIN_WAVES, top ? 4 * (groups + (top < groups ? top : groups) * LP_GROUP) : 0, stream>>>(logits, stride, V, shares, share, tops, groups, ids, logprob, entropy, top, top_ids, top_logprob);
     return li_launch_status();
 }

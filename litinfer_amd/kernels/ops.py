@@ -1941,6 +1941,7 @@ def sample_prepare(rows: torch.Tensor, table: torch.Tensor, temperature: torch.T
 # ------------------------------------------------------------------ log probabilities of given tokens
 LOGPROBS_MAX_TOP = 32                  # alternatives a row
 LOGPROBS_MAX_VOCAB = 1 << 20
+LOGPROBS_MAX_ROWS = 1 << 30
 
 
 def _here(what: str, *ts) -> None:
@@ -1976,6 +1977,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tens
         top = shape[1]
         if top > LOGPROBS_MAX_TOP or top > v:
             _chk(False, f"token_logprobs: {top} alternatives of {v} tokens (at most {LOGPROBS_MAX_TOP})")
+    if n > LOGPROBS_MAX_ROWS:
+        _chk(False, f"token_logprobs: {n} rows (at most 2^30)")
     if not 0 < v <= LOGPROBS_MAX_VOCAB:
         _chk(False, f"token_logprobs: rows of {v} logits (1 to {LOGPROBS_MAX_VOCAB})")
     if n:

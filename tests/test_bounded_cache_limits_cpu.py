@@ -59,3 +59,12 @@ def test_the_library_refuses(max_blocks, page_size, K):
         one = (ops.c_int * 1)(1)
         at = ops.ctypes.addressof(one)
         assert ops._fn("evict", "li_attention_mass")(0, 64, 0, 0, 0, 0, max_blocks, 0, 0, 0, at, at, at, 1, 1, 0, 4, 2, 8, page_size, 9, 1.0, 1, at, 1 << 20, 0) == REFUSED
+
+
+@pytest.mark.parametrize("rows", [MANY, (1 << 31) - 1, (1 << 32) + 5])
+def test_token_logprobs_refuses(no_gpu, rows):  # noqa: F811
+    with pytest.raises(ValueError, match="token_logprobs: .* rows .*2.30"):
+        ops.token_logprobs(f32(rows, 2), i32(rows), f32(rows), f32(rows))
+    if rows < 1 << 31:
+        one = (ops.c_int * 1)(1)
+        assert ops._fn("logprobs", "li_token_logprobs")(0, 2, 0, rows, 2, 0, 0, 0, 0, 0, ops.ctypes.addressof(one), 0) == REFUSED
