@@ -302,9 +302,6 @@ extern "C" long li_token_logprobs_work_floats(int n, int V) {
     return (long)n * (4L * row_shares(V, share_groups(n)) + groups_of(V));
 }
 
-extern "C" int li_token_logprobs_max_top(void) { return LP_MAX_TOP; }
-extern "C" int li_token_logprobs_max_vocab(void) { return LP_MAX_GROUPS * LP_GROUP; }
-
 // logits [n, V], rows `stride` floats apart; ids [n]; logprob, entropy [n]; top_ids, top_logprob [n, top] (top 0: none).  An id
 // outside the row has no probability (NaN).
 extern "C" int li_token_logprobs(const float* logits, long stride, const int* ids, int n, int V, int top, float* logprob, float* entropy,

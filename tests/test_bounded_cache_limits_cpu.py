@@ -68,3 +68,11 @@ def test_token_logprobs_refuses(no_gpu, rows):  # noqa: F811
     if rows < 1 << 31:
         one = (ops.c_int * 1)(1)
         assert ops._fn("logprobs", "li_token_logprobs")(0, 2, 0, rows, 2, 0, 0, 0, 0, 0, ops.ctypes.addressof(one), 0) == REFUSED
+
+
+def test_the_limits_that_python_names_are_the_library_s():
+    """One more is refused by the library; the limits themselves are taken by the tests on the GPU (32 alternatives) or by their arithmetic."""
+    one = (ops.c_int * 1)(1)
+    call = ops._fn("logprobs", "li_token_logprobs")
+    for v, top in ((ops.LOGPROBS_MAX_VOCAB + 1, 0), (99, ops.LOGPROBS_MAX_TOP + 1)):
+        assert call(0, 1 << 22, 0, 1, v, top, 0, 0, 0, 0, ops.ctypes.addressof(one), 0) == REFUSED
