@@ -2000,6 +2000,7 @@ def attention_mass(qkv: torch.Tensor, mass: torch.Tensor, k: torch.Tensor, meta,
     `paged_attention` takes it (a query sees the keys up to its own place), no page in two of its requests; mass [pages, nkv, page_size, 1] float32
     lies in the keys' pages.  With
     `fresh` the sums of the keys that this step wrote begin at zero (whatever the pages held); an entry that reads another's keys adds to all.
+    A query that sees no page, or none but keys whose scores are -inf, adds nothing; one that sees a score of NaN or +inf makes the sums of all its keys NaN.
     Sums are float32 in an order that depends on the batch alone.  Recorded into a graph, a batch that is not `padded` keeps the lengths that it
     was recorded with.  `ws` lends the buffers."""
     bt = meta.block_table
