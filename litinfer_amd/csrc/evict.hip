@@ -67,7 +67,7 @@ __device__ __forceinline__ long some_row(const MassArgs& a, const int* table, in
 }
 
 // ---- any head size, type and alignment: scores by the vector ALU, computed twice.  Nothing here is made for speed: rows of whole 16 bytes on 16 bytes, which
-// models have, go the other ways.
+// models have, go the other ways.  (14 heads on 2 of 36 bfloat16: 8 requests of 2,000 keys 64 us; 512 queries behind 2,048 keys 2.7 ms, where heads of 64 take 29 us.)
 template <typename T>
 __device__ __forceinline__ float dot_rows(const float* q, const T* k, int dh) {
     float s = 0.f;
@@ -164,7 +164,8 @@ __device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x
 // ---- single tokens.  The scores themselves are kept (4 bytes a query head and key beside the key's dh * 2): reading the keys
 // again would cost more.  Bound by the keys' way from memory and, at these sizes, by the launches around it: 64 requests of 100 to 2,001 keys, 12 heads on 2 of 128
 // bfloat16 (36 MB), 13.8 us for the scores and 5.3 for the sums; 3 of 20,000 to 32,001 keys, 28 heads on 4 of 128 float32 (162 MB), 39.6 (4.0 TB/s) and 12.1; one
-// of 300 keys, 14 heads on 2, 6.2 in one kernel.
+// of 300 keys, 14 heads on 2, 6.2 in one kernel.  A recorded step lays its scores out for the whole tables: 28 heads on 4 of 128 bfloat16, 8 requests of
+// 4,000 keys 15.6 in tables of 4,096 places and 23.1 in tables of 32,768 (named, 15.5), 64 of 1,000 in tables of 4,096 58 (named, 16.4).
 #define SG_KEYS 64                // keys of a wave
 #define SG_WAVES 4
 // Floats of workspace that the requests of a launch take together, unless one takes more by itself: a batch beyond that goes in several launches, one
@@ -355,8 +356,10 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
 }
 
 // ---- portions: tiles of 32 x 32 scores.  One side's rows stay in a wave's registers (ST tiles of 32 rows a wave), the other's go
-// through LDS in stages of 64 rows (32 where three of 64 do not fit).  Loads go straight into LDS; a stage is asked for while the one before
-// the last is worked on.  A row's pieces are swizzled (place p of row r holds piece p ^ (r & 15)), so that rows' pieces of one column lie
+// through LDS in stages of 64 rows (32 where three of 64 do not fit).  Loads go straight into LDS.  The columns' pass asks for a stage while the one before
+// the last is worked on; the rows' pass asks for it then too, but waits for it at once: the table's entry for the stage behind it (look_up) is a load
+// like any other, asked for last and wanted first, and loads arrive in order.  So its third stage in LDS gains it nothing, and the rows' pass takes
+// a sixth longer than the columns' for the same products.  A row's pieces are swizzled (place p of row r holds piece p ^ (r & 15)), so that rows' pieces of one column lie
 // in different banks.
 //
 // A step is one tile of 32 staged rows: its products, beside them the exponentials of the tile before (MFMAs and the vector ALU work side by
@@ -855,7 +858,9 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
         const long lds = 4 * (rep * (SG_KEYS + 2L) * p.parts + rep);
         // One kernel where a block has few keys, or where the blocks fill the compute units, us: bfloat16, 28 heads on 4 of 128, one request of 300 keys 9.0
         // (two kernels) and 6.8, 64 requests 13.3 and 7.1, of 1,000 20.0 and 14.8, of 2,000 32.5 and 25.6; 8 requests of 1,000 9.4 and 12.8, 64
-        // of 2,000 on 2 kv heads 20.3 and 23.5.
+        // of 2,000 on 2 kv heads 20.3 and 23.5.  Recorded steps are asked about the tables' room, not the contexts; one kernel and two, us: 28 heads on 4, one
+        // request of 500 in 512 places 8.7 and 9.6, of 1,000 in 1,024 13.0 and 9.6, 64 of 1,000 in 1,024 16.5 and 23.1, of 2,000 in 2,048 32.4 and 41.5; 8 of 1,000 in 1,024 14.0
+        // and 10.8; 12 heads on 2 (128 blocks: two kernels), 64 of 1,100 in 2,048 15.8 and 20.0, of 2,000 25.1 and 22.0.
         p.one_block = lds <= 150 * 1024 && (p.device_ctx <= 512 || ((long)p.single * nkv >= 192 && p.device_ctx <= 2048));
         p.block_lds = (int)lds;
         // a mix, or few: they are named, and their lengths need no trip to memory
@@ -870,7 +875,9 @@ static MassPlan mass_plan(const int* q_len, const int* ctx_len, int nseg, int to
         // some length, else one, and there are more of them.  Rows: two from 16 stages a block on.  Keys: two from 20 pairs a block on; one and two, us of both
         // passes: a prompt of 2,048 of 28 heads on 4 79 and 87, of 512 of 14 heads on 2 21 and 26, 990 of 12 heads on 2 behind 500 33 and 36, 4 x 512 of 28
         // heads behind 1,000 68 and 78 (8 to 14 pairs); 2,048 behind 2,000 149 and 149 (21); a prompt of 4,000 of 28 heads 195 and 191 (28), 2,048 behind
-        // 8,000 375 and 334, 1,999 of 40 heads on 8 behind 16,000 850 and 788 (166).
+        // 8,000 375 and 334, 1,999 of 40 heads on 8 behind 16,000 850 and 788 (166).  float32, whose rows take twice the registers: one tile always; one and two, us of both
+        // passes: a prompt of 2,048 of 28 heads on 4 of 128 379 and 470, 512 of 14 heads on 2 of 64 behind 2,048 73 and 98, 2,048 of the same behind 8,192 691 and 736, but 512 of 28
+        // heads behind 4,096 377 and 312.
         const int rows = 32 * stage_tiles((dh <= 64 ? 64 : dh <= 128 ? 128 : 256) * (f32 ? 4 : 2));
         for (p.row_st = f32 ? 1 : 2;; p.row_st = 1) {
             long stages = 0, most = 0, all = 0;
@@ -1221,7 +1228,9 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(SelectArgs a) {
 
 #define SEL_NT 1024
 
-// Requests that are longer than a block's registers: the sums are read again for every digit, eight bits of them, the digits counted in LDS.
+// Requests that are longer than a block's registers: the sums are read again for every digit, eight bits of them, the digits counted in LDS.  (The digits are
+// the leading bits of the floats' order, of which sums within a few octaves share most: many lanes add to one counter.)  Bound by that and by five
+// passes of one block over the list: one request of 40,000 places, 8 entries x 8 kv heads 156 us, of 130,000 599; 28 x 4 208 and 601.
 __global__ __launch_bounds__(SEL_NT) void evict_select_long_kernel(SelectArgs a) {
     __shared__ int hist[256], wsum[SEL_NT / 64], pick[2];
     const int kvh = blockIdx.x, req = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;

@@ -124,7 +124,9 @@ __device__ __forceinline__ int block_count(int n, int (*smem)[LP_JOIN_WAVES], in
 // One block a row: joins the waves' shares, then finds the likeliest tokens.  A value that at least k and at most LP_LIST groups' maxima
 // reach is found by halving the range between the least and the largest; the logits of these groups that reach it are gathered (at least
 // k, seldom many more) and each one's rank counted.  Where many values are equal or likely tokens lie side by side no such value may exist, or more
-// logits reach it than there is room for: then the k first are taken one after the other.  A chain of short steps with a barrier behind each: eight waves
+// logits reach it than there is room for: then the k first are taken one after the other.  So they are in every row of few groups, of which no more are wanted than
+// there are (`enough`, 30 for 20 alternatives: up to 7,680 logits; 48 for 32): there all logits reach.  (64 rows with 20 alternatives, us of both kernels: 3,001 logits 32,
+// 7,500 42, 8,000 12.)  A chain of short steps with a barrier behind each: eight waves
 // take 9.2 us for a row with 20 alternatives (both kernels), four 11.3, sixteen 9.0; at 2,047 rows 242, 242 and 256.
 #define LP_LIST 64                // groups that are looked through
 #define LP_ROOM 256               // logits that are ranked
