@@ -165,15 +165,16 @@ __device__ __forceinline__ f32x16_t mma32(const u32x4_t a, const u32x4_t b, f32x
 // again would cost more.  Bound by the keys' way from memory and, at these sizes, by the launches around it: 64 requests of 100 to 2,001 keys, 12 heads on 2 of 128
 // bfloat16 (36 MB), 13.8 us for the scores and 5.3 for the sums; 3 of 20,000 to 32,001 keys, 28 heads on 4 of 128 float32 (162 MB), 39.6 (4.0 TB/s) and 12.1; one
 // of 300 keys, 14 heads on 2, 6.2 in one kernel.  A recorded step lays its scores out for the whole tables: 28 heads on 4 of 128 bfloat16, 8 requests of
-// 4,000 keys 15.6 in tables of 4,096 places and 23.1 in tables of 32,768 (named, 15.5), 64 of 1,000 in tables of 4,096 58 (named, 16.4).
+// 4,000 keys 15.6 in tables of 4,096 places and 22.4 in tables of 32,768 (named, 15.4), 64 of 1,000 in tables of 4,096 57.5 (named, one kernel, 16.6).
 #define SG_KEYS 64                // keys of a wave
 #define SG_WAVES 4
 // Floats of workspace that the requests of a launch take together, unless one takes more by itself: a batch beyond that goes in several launches, one
 // after the other, which use it again.  (256 MiB: more work than fills the chip many times over.)
 #define SG_ROOM (1L << 26)
 
-// A request's scores [heads, 64 parts] and behind them the statistics [heads, parts] (maximum, sum), in whole 16 bytes.
-__host__ __device__ __forceinline__ long single_floats(int nh, int parts) { return ((long)nh * parts * (SG_KEYS + 2) + 3) / 4 * 4; }
+// A request's scores [heads, 64 parts] and behind them the statistics (maximum, sum) [heads, parts], a head's in whole lines of 128 bytes.
+constexpr int stat_stride(int parts) { return (parts + 15) & ~15; }
+static long single_floats(int nh, int parts) { return nh * (parts * (long)SG_KEYS + 2 * stat_stride(parts)); }
 
 // Scores of the 64 keys from k0 on against the heads of a kv head, 16 at a time, by a wave, and the maximum and sum for every head:
 // scores [head of the kv head, stride] from key k0 on, stats [head, parts].
@@ -241,26 +242,21 @@ __device__ __forceinline__ void single_scores(const T* __restrict__ qrow, const 
     }
 }
 
-// Where a request's scores lie: those that are listed side by side, each as long as it is; others, from segment `first` on, `parts` runs of 64 each.
-struct Single {
-    int seg, start, ctx, parts;
+// A launch's request `req`: from the list, or the segment `first` + req (then without its row, which only blocks with keys ask for).
+__device__ __forceinline__ Seg single_of(const MassArgs& a, const SegList& list, int req, int first, int parts) {
+    if (list.n) return list.of[req];
+    return {first + req, -1, 1, device_ctx(a, first + req, parts * SG_KEYS), 0};
+}
+// Where its scores lie: those of listed requests side by side, each as long as it is, of others `parts` runs of 64, `each` floats.
+struct Scores {
+    int parts;
     float* scores;
     float2* stats;
 };
-__device__ __forceinline__ Single single_of(const MassArgs& a, const SegList& list, int req, int first, int parts, float* work) {
-    Single s;
-    if (list.n) {
-        const Seg of = list.of[req];
-        s.seg = of.seg; s.start = of.start; s.ctx = of.ctx;
-        s.parts = (of.ctx + SG_KEYS - 1) / SG_KEYS;
-        s.scores = work + of.off;
-    } else {
-        s.seg = first + req;
-        s.start = a.q_start[s.seg];
-        s.ctx = device_ctx(a, s.seg, parts * SG_KEYS);
-        s.parts = parts;
-        s.scores = work + req * single_floats(a.nh, parts);
-    }
+__device__ __forceinline__ Scores scores_of(const MassArgs& a, const SegList& list, const Seg& of, int req, int parts, long each, float* work) {
+    Scores s;
+    s.parts = list.n ? (of.ctx + SG_KEYS - 1) / SG_KEYS : parts;
+    s.scores = work + (list.n ? (long)of.off : req * each);
     s.stats = reinterpret_cast<float2*>(s.scores + (size_t)a.nh * s.parts * SG_KEYS);
     return s;
 }
@@ -268,16 +264,17 @@ __device__ __forceinline__ Single single_of(const MassArgs& a, const SegList& li
 // grid: x runs of 64 keys / 4, y kv heads, z requests.
 template <typename T, int CH>
 __global__ __launch_bounds__(64 * SG_WAVES) void mass_single_scores_kernel(const T* __restrict__ q, const T* __restrict__ k, MassArgs a, SegList list,
-                                                                           int first, float* __restrict__ work, int parts) {
+                                                                           float* __restrict__ work, long each, int first, int parts) {
     const int req = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, rep = a.nh / a.nkv;
     const int k0 = (blockIdx.x * SG_WAVES + (threadIdx.x >> 6)) * SG_KEYS;
-    const Single s = single_of(a, list, req, first, parts, work);
-    if (k0 >= s.ctx) return;
-    const T* qrow = q + (size_t)s.start * a.q_row_stride + (size_t)kvh * rep * a.dh;
+    const Seg of = single_of(a, list, req, first, parts);
+    if (k0 >= of.ctx) return;
+    const Scores s = scores_of(a, list, of, req, parts, each, work);
+    const T* qrow = q + (size_t)(list.n ? of.start : a.q_start[of.seg]) * a.q_row_stride + (size_t)kvh * rep * a.dh;
     const size_t head0 = (size_t)kvh * rep;
     const long stride = (long)s.parts * SG_KEYS;
-    single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)s.seg * a.max_blocks, kvh, k0, s.ctx, lane, s.scores + head0 * stride, stride, s.stats + head0 * s.parts,
-                         s.parts);
+    single_scores<T, CH>(qrow, k, a, a.block_table + (size_t)of.seg * a.max_blocks, kvh, k0, of.ctx, lane, s.scores + head0 * stride, stride, s.stats + head0 * stat_stride(s.parts),
+                         stat_stride(s.parts));
 }
 
 // lse of a head from the statistics of its `n` parts, by a wave.
@@ -329,14 +326,15 @@ __global__ __launch_bounds__(64 * block_waves(CH)) void mass_single_block_kernel
 }
 
 #define SG_LSE 64                 // heads of a kv head whose lse a block holds at a time
-__global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegList list, int first, float* __restrict__ work, int parts, float* __restrict__ mass) {
+__global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegList list, float* __restrict__ work, long each, int first, int parts, float* __restrict__ mass) {
     __shared__ float lse[SG_LSE];
     const int req = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = blockIdx.x * 256 + threadIdx.x, rep = a.nh / a.nkv;
-    const Single s = single_of(a, list, req, first, parts, work);
-    const int ctx = s.ctx;
+    const Seg of = single_of(a, list, req, first, parts);
+    const int ctx = of.ctx;
     if ((int)blockIdx.x * 256 >= ctx) return;
+    const Scores s = scores_of(a, list, of, req, parts, each, work);
     const int n = (ctx + SG_KEYS - 1) / SG_KEYS;
-    const long row = t < ctx ? place_row(a, a.block_table + (size_t)s.seg * a.max_blocks, kvh, t) : -1;
+    const long row = t < ctx ? place_row(a, a.block_table + (size_t)of.seg * a.max_blocks, kvh, t) : -1;
     const float before = row >= 0 && !(a.fresh && t == ctx - 1) ? mass[row] : 0.f;
     const size_t head0 = (size_t)kvh * rep;
     const long stride = (long)s.parts * SG_KEYS;
@@ -345,7 +343,7 @@ __global__ __launch_bounds__(256) void mass_single_add_kernel(MassArgs a, SegLis
         const int heads = min(rep - h0, SG_LSE);
         __syncthreads();
         for (int h = w; h < heads; h += 4) {
-            const float v = join_stats(s.stats + (head0 + h0 + h) * s.parts, n, lane);
+            const float v = join_stats(s.stats + (head0 + h0 + h) * stat_stride(s.parts), n, lane);
             if (lane == 0) lse[h] = v;
         }
         __syncthreads();
@@ -951,8 +949,8 @@ static int launch_mass_tiled(const T* q, const T* k, float* mass, const MassArgs
                 block<<<dim3(a.nkv, now.n), 64 * block_waves(CH16), p.block_lds, stream>>>(q, k, a, list, p.parts * SG_KEYS, mass);
             } else {
                 mass_single_scores_kernel<T, CH16><<<dim3((now.parts + SG_WAVES - 1) / SG_WAVES, a.nkv, now.n), 64 * SG_WAVES, 0, stream>>>(
-                    q, k, a, list, at, work, now.parts);
-                mass_single_add_kernel<<<dim3((now.parts + 3) / 4, a.nkv, now.n), 256, 0, stream>>>(a, list, at, work, now.parts, mass);
+                    q, k, a, list, work, single_floats(a.nh, now.parts), at, now.parts);
+                mass_single_add_kernel<<<dim3((now.parts + 3) / 4, a.nkv, now.n), 256, 0, stream>>>(a, list, work, single_floats(a.nh, now.parts), at, now.parts, mass);
             }
             at += now.n;
         }

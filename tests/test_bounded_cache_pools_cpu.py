@@ -202,8 +202,9 @@ ROOM = 1 << 26                                                    # floats that 
 
 
 def scores(nh, ctx):
-    """What a request's scores and statistics take, in whole 16 bytes."""
-    return -(-nh * -(-ctx // 64) * 66 // 4) * 4
+    """What a request's scores take in runs of 64 keys, and a run's statistics, 16 of them in a line."""
+    runs = -(-ctx // 64)
+    return nh * (64 * runs + 2 * 16 * -(-runs // 16))
 
 
 def test_the_workspace_of_single_tokens_goes_by_what_each_has_cached():
