@@ -17,7 +17,7 @@ import os
 import sys
 from collections import OrderedDict
 from pathlib import Path
-from typing import Any, Dict, Hashable, List, Optional, Sequence
+from typing import Any, Dict, Hashable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -47,6 +47,7 @@ def parse_dtype(dtype) -> torch.dtype:
 
 
 FEEDBACK_SLOTS = 4096
+EVICT_ROOM = 1 << 28                  # bytes that the lists of an eviction's kept places take together
 
 
 class StepError(ValueError):
@@ -355,26 +356,33 @@ class Engine:
         cache = self.cache
         held = {rid: cache.cached_len(rid) for rid in rids}          # (an unknown request: KeyError)
         longer = [rid for rid in rids if held[rid] > keep]
-        if longer:
-            from ..kernels import ops
-            n = len(longer)
-            tables = []
-            for g in range(len(cache.groups)):
-                rows = [cache.block_table(rid, g) for rid in longer]
-                table = np.full((n, max(map(len, rows))), -1, dtype=np.int32)
-                for row, ids in zip(table, rows):
-                    row[:len(ids)] = ids
-                tables.append(table)
-            up = self._evict_up.upload([np.array([held[r] for r in longer], dtype=np.int32), np.full(n, keep, dtype=np.int32), *tables])
-            kept = []
-            for group, table in zip(cache.groups, up[2:]):
-                mass = group.data["mass"]
-                kept.append(torch.empty((mass.shape[0], n, mass.shape[2], keep), dtype=torch.int32, device=mass.device))
-                ops.evict_select(mass, table, up[0], up[1], first, recent, kept[-1])
-            for group, table, places in zip(cache.groups, up[2:], kept):
-                ops.cache_compact(list(group.data.values()), table, places)
-            cache.evict_many(cache.handles_of(longer), keep)
+        # (the places that stay are listed for every layer and kv head: many long requests go some at a time)
+        places = sum(g.data["mass"].shape[0] * g.data["mass"].shape[2] for g in cache.groups) * keep
+        at_once = max(1, EVICT_ROOM // (4 * places))
+        for at in range(0, len(longer), at_once):
+            self._evict([(rid, held[rid]) for rid in longer[at:at + at_once]], keep, first, recent)
         return [min(held[rid], keep) for rid in rids]
+
+    def _evict(self, longer: Sequence[Tuple[Hashable, int]], keep: int, first: int, recent: int) -> None:
+        """Cuts requests, given with their cached lengths, all of which hold more than `keep` tokens."""
+        from ..kernels import ops
+        cache, n = self.cache, len(longer)
+        tables = []
+        for g in range(len(cache.groups)):
+            rows = [cache.block_table(rid, g) for rid, _ in longer]
+            table = np.full((n, max(map(len, rows))), -1, dtype=np.int32)
+            for row, ids in zip(table, rows):
+                row[:len(ids)] = ids
+            tables.append(table)
+        up = self._evict_up.upload([np.array([held for _, held in longer], dtype=np.int32), np.full(n, keep, dtype=np.int32), *tables])
+        kept = []
+        for group, table in zip(cache.groups, up[2:]):
+            mass = group.data["mass"]
+            kept.append(torch.empty((mass.shape[0], n, mass.shape[2], keep), dtype=torch.int32, device=mass.device))
+            ops.evict_select(mass, table, up[0], up[1], first, recent, kept[-1])
+        for group, table, places in zip(cache.groups, up[2:], kept):
+            ops.cache_compact(list(group.data.values()), table, places)
+        cache.evict_many(cache.handles_of([rid for rid, _ in longer]), keep)
 
     def finish(self, rid: Hashable) -> None:
         """The request is over: what it holds is given back."""

@@ -10,7 +10,7 @@ import bounded_cache_cases as cases
 import helpers
 import plain_impl
 from litinfer_amd.cache import CacheFull
-from litinfer_amd.engine import Engine, Scheduler
+from litinfer_amd.engine import Engine, Scheduler, StepEntry
 from litinfer_amd.engine.workspace import Workspace
 from litinfer_amd.kernels import ops
 from litinfer_amd.models import Qwen2
@@ -248,3 +248,27 @@ def test_what_the_sums_take_is_set_aside_before_the_pages_are_counted(bounded_op
     # (the buffer that is too small and the one that takes its place: 4 bytes a float, grown by half)
     assert a._page_memory(free) <= 0.85 * (free - 4 * (ROOM + ROOM * 3 // 2)) and a._page_memory(free) > 0.84 * free
     assert a._page_memory(1 << 30) == int((1 << 29) * 0.85)
+
+
+@pytest.mark.parametrize("requests", [4, 2, 1, 0])
+def test_evictions_of_many_long_requests_go_some_at_a_time(bounded_ops, model, monkeypatch, requests):
+    """20 of 30 to 60 tokens stay, listed for each of the model's layers and kv heads, 4 bytes each."""
+    from litinfer_amd.engine import engine as module
+    layers, heads = CFG["num_hidden_layers"], CFG["num_key_value_heads"]
+    monkeypatch.setattr(module, "EVICT_ROOM", requests * 4 * layers * heads * 20)
+    lists = []
+    select = ops.evict_select
+    monkeypatch.setattr(ops, "evict_select", lambda *a: lists.append(a[-1].shape) or select(*a))
+    eng, alone = engine(model, num_pages=100), engine(model, num_pages=100)
+    names = [f"r{i}" for i in range(4)]
+    for e in (eng, alone):
+        for i, rid in enumerate(names):
+            e.step([StepEntry(rid, text(30 + 10 * i, i), [])])
+    assert eng.evict(names, 20) == [20] * 4
+    assert [shape[1] for shape in lists] == [max(1, requests)] * (4 // max(1, requests))
+    for rid in names:
+        alone.evict([rid], 20)
+    eng.cache.check_invariants()
+    for rid in names:
+        step = [StepEntry(rid, [7], [0])]
+        assert torch.equal(eng.step(step), alone.step(step))
